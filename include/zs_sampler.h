@@ -39,7 +39,7 @@
 extern "C" {
 #endif
 
-#define ZS_ABI_VERSION 4
+#define ZS_ABI_VERSION 5
 
 typedef enum zs_status {
     ZS_OK = 0,
@@ -293,6 +293,121 @@ zs_status zs_set_small_batch(zs_handle h, int32_t max_rows);
 zs_status zs_logits_stats(zs_handle h, const float* logits, int64_t ld, int32_t batch,
                           int32_t n_vocab, int32_t topn, double* out_min, double* out_max,
                           double* out_z, int32_t* top_ids, double* top_p, void* stream);
+
+/* ---------------------------------------------------------------------------------
+ * Log probabilities and the embedding table: what a caller needs on both sides of the
+ * sampler (scoring, policy-gradient or cross-entropy training, the next step's input).
+ * No counterpart in the reference, which only samples.  These calls use no handle
+ * scratch: where one needs a workspace the caller passes it, so calls on different
+ * streams (each with its own workspace) and captured graphs do not disturb each other.
+ * zs_set_timing counts their launches but does not time them.
+ * --------------------------------------------------------------------------------- */
+#define ZS_DTYPE_F32 0
+#define ZS_DTYPE_F16 1
+#define ZS_DTYPE_BF16 2
+#define ZS_LOGPROBS_MAX_TOP 128
+#define ZS_LOGPROBS_MAX_IDS 256
+#define ZS_EMBED_MAX_TOKENS (1 << 30)
+#define ZS_EMBED_MAX_EMBD (1 << 20)
+
+/* What zs_logprobs_backward needs of a row (16 bytes). */
+typedef struct zs_logprob_row {
+    float max;      /* the row's largest logit */
+    float sum;      /* sum of exp((x - max) * inv_temp); 0 when every logit is -inf */
+    float entropy;
+    float inv_temp; /* 1 / temp (1 for temp <= 0) */
+} zs_logprob_row;
+
+/*
+ * With p = softmax(x / temp) over each of `batch` rows of n_vocab logits (`dtype`, row r
+ * at logits + r * ld elements, any alignment of the type, never modified):
+ *   out_logp     device [batch][n_ids]: log p of the given ids (ids: device
+ *                [batch][ids_ld], the first n_ids of a row; 0 to ZS_LOGPROBS_MAX_IDS);
+ *                0 for an id outside [0, n_vocab), such as the -1 of a stopped row of
+ *                zs_decode_step
+ *   top_ids      device [batch][topn]: the k = min(topn, n_vocab) largest logits, value
+ *                descending then id ascending (0 to ZS_LOGPROBS_MAX_TOP), and
+ *   top_logp     their log p; entries k .. topn - 1 are left as they were
+ *   out_entropy  device [batch], optional: -sum p log p
+ *   out_lse      device [batch], optional: log sum exp(x / temp)
+ *   out_rows     device [batch] (16-byte aligned), optional: for zs_logprobs_backward
+ * row_temp (device [batch]) gives every row its own temperature, or is NULL and temp
+ * holds for all.  temp <= 0 counts as 1, as for row_info.log_z; 1 / temp is taken in f32
+ * as the sampler takes it.  The sums are f32, the values of a row's ids f64 up to the
+ * last rounding.
+ * A logit of -inf is a masked token: p = 0 and log p = -inf.  A row of -inf only has
+ * lse = -inf, log p = -inf and entropy 0.  NaN or +inf in a row makes its numbers NaN;
+ * its top_ids keep their order (NaN after -inf).
+ */
+zs_status zs_logprobs(zs_handle h, const void* logits, int32_t dtype, int64_t ld, int32_t batch,
+                      int32_t n_vocab, float temp, const float* row_temp, const int32_t* ids,
+                      int64_t ids_ld, int32_t n_ids, float* out_logp, int32_t topn,
+                      int32_t* top_ids, float* top_logp, float* out_entropy, float* out_lse,
+                      zs_logprob_row* out_rows, void* stream);
+
+/*
+ * The gradient with respect to the logits of
+ *   sum_j grad_logp[r][j] log p[ids[r][j]] + grad_entropy[r] entropy[r] + grad_lse[r] lse[r]
+ * for every row (lse that of x / temp), from the logits and out_rows of zs_logprobs:
+ *   grad_logits  device, `dtype`, row r at grad_logits + r * grad_ld; may be the logits'
+ *                own buffer (grad_ld = ld)
+ *   grad_logp    device [batch][n_ids]; grad_entropy, grad_lse device [batch] or NULL
+ * Equal ids in a row add up; ids outside [0, n_vocab) give nothing.  Rows of -inf only
+ * get 0.  Every element is computed in f32 and rounded once.
+ */
+zs_status zs_logprobs_backward(zs_handle h, const void* logits, int32_t dtype, int64_t ld,
+                               int32_t batch, int32_t n_vocab, const zs_logprob_row* rows,
+                               const int32_t* ids, int64_t ids_ld, int32_t n_ids,
+                               const float* grad_logp, const float* grad_entropy,
+                               const float* grad_lse, void* grad_logits, int64_t grad_ld,
+                               void* stream);
+
+/*
+ * zs_logprobs of the logits that zs_lmhead_logits computes on the tensor cores
+ * (logits = rmsnorm(hidden, norm_w, eps) rounded to bf16 . weight^T, f32 accumulation,
+ * at every batch size), without the logits in memory: the statistics are taken in the
+ * GEMM's epilogue.  Arguments as there; no top alternatives, and for inference: to
+ * train, take zs_lmhead_logits, zs_logprobs and zs_logprobs_backward.
+ *   workspace  device, 256-byte aligned, at least zs_lmhead_logprobs_workspace bytes
+ *              (which follow zs_set_lmhead_tiles)
+ * A wait that runs out is reported by zs_check_device_status.
+ */
+zs_status zs_lmhead_logprobs_workspace(zs_handle h, int32_t batch, int32_t n_embd, int32_t n_vocab,
+                                       int64_t* out_bytes);
+zs_status zs_lmhead_logprobs(zs_handle h, const float* hidden, int64_t hidden_ld,
+                             const float* norm_w, float eps, const void* weight, int32_t batch,
+                             int32_t n_embd, int32_t n_vocab, float temp, const float* row_temp,
+                             const int32_t* ids, int64_t ids_ld, int32_t n_ids, float* out_logp,
+                             float* out_entropy, float* out_lse, void* workspace,
+                             int64_t workspace_bytes, void* stream);
+
+/*
+ * out[i] = scale * table[ids[i]] for n_tokens ids (device int32), e.g. the out_ids of
+ * zs_decode_step and the lm_head's own weights where the two are tied.  table: device
+ * [n_vocab][table_ld], out: device [n_tokens][out_ld], the first n_embd columns of a
+ * row; each of its own type.  An id outside [0, n_vocab) (-1: a stopped row) gives a
+ * row of zeros.  The product is f32, rounded once.
+ */
+zs_status zs_embed(zs_handle h, const void* table, int32_t table_dtype, int64_t table_ld,
+                   int32_t n_vocab, int32_t n_embd, const int32_t* ids, int64_t n_tokens,
+                   float scale, void* out, int32_t out_dtype, int64_t out_ld, void* stream);
+
+/*
+ * The gradient of zs_embed's table: grad_table[v] = scale * sum of grad_out[i] over the
+ * i with ids[i] == v, and 0 for an id that does not occur (accumulate = 0), or added to
+ * grad_table (accumulate != 0, which leaves the rows of other ids alone).  The rows of
+ * an id are summed in f32 in a fixed order, so equal calls give equal bits, and each
+ * element is rounded to grad_table's type once.  Columns n_embd .. table_ld - 1 are
+ * left alone.
+ *   workspace  device, 256-byte aligned, at least zs_embed_backward_workspace bytes
+ *              (may be NULL when n_tokens is 0)
+ */
+zs_status zs_embed_backward_workspace(int64_t n_tokens, int32_t n_embd, int64_t* out_bytes);
+zs_status zs_embed_backward(zs_handle h, const void* grad_out, int32_t grad_dtype, int64_t grad_ld,
+                            const int32_t* ids, int64_t n_tokens, float scale, int32_t n_vocab,
+                            int32_t n_embd, void* grad_table, int32_t table_dtype,
+                            int64_t table_ld, int32_t accumulate, void* workspace,
+                            int64_t workspace_bytes, void* stream);
 
 /* ---------------------------------------------------------------------------------
  * Vocab-sharded sampling (tensor-parallel lm_head layout).  Rank g of n_ranks

@@ -21,7 +21,9 @@ EXPORTS = (
     "zs_selftest_wait_timeout", "zs_decode_step", "zs_lmhead_sample", "zs_lmhead_logits",
     "zs_set_lmhead_route", "zs_shard_owner_rows", "zs_shard_row_spans", "zs_shard_merge_rows",
     "zs_set_collective_timeout", "zs_set_speculation", "zs_set_small_batch",
-    "zs_set_lmhead_tiles",
+    "zs_set_lmhead_tiles", "zs_logprobs", "zs_logprobs_backward", "zs_lmhead_logprobs",
+    "zs_lmhead_logprobs_workspace", "zs_embed", "zs_embed_backward",
+    "zs_embed_backward_workspace",
 )
 
 ZS_OK = 0
@@ -108,6 +110,18 @@ def lib() -> C.CDLL:
     L.zs_get_timing.argtypes = [vp, C.POINTER(ZsTiming)]
     L.zs_sample_noalloc.argtypes = [vp, i64, i32, i32, C.POINTER(ZsParams), vp, i64, vp, vp, vp,
                                     vp, vp]
+    f32 = C.c_float
+    L.zs_logprobs.argtypes = [vp, vp, i32, i64, i32, i32, f32, vp, vp, i64, i32, vp, i32, vp, vp,
+                              vp, vp, vp, vp]
+    L.zs_logprobs_backward.argtypes = [vp, vp, i32, i64, i32, i32, vp, vp, i64, i32, vp, vp, vp,
+                                       vp, i64, vp]
+    L.zs_lmhead_logprobs_workspace.argtypes = [vp, i32, i32, i32, C.POINTER(i64)]
+    L.zs_lmhead_logprobs.argtypes = [vp, vp, i64, vp, f32, vp, i32, i32, i32, f32, vp, vp, i64,
+                                     i32, vp, vp, vp, vp, i64, vp]
+    L.zs_embed.argtypes = [vp, vp, i32, i64, i32, i32, vp, i64, f32, vp, i32, i64, vp]
+    L.zs_embed_backward_workspace.argtypes = [i64, i32, C.POINTER(i64)]
+    L.zs_embed_backward.argtypes = [vp, vp, i32, i64, vp, i64, f32, i32, i32, vp, i32, i64, i32,
+                                    vp, i64, vp]
     for name in EXPORTS:
         f = getattr(L, name)
         if f.restype is C.c_int or name in ("zs_create", "zs_destroy", "zs_sample", "zs_argmax",
@@ -121,7 +135,10 @@ def lib() -> C.CDLL:
                                             "zs_shard_owner_rows", "zs_shard_row_spans",
                                             "zs_shard_merge_rows", "zs_set_collective_timeout",
                                             "zs_set_speculation", "zs_set_small_batch",
-                                            "zs_set_lmhead_tiles"):
+                                            "zs_set_lmhead_tiles", "zs_logprobs",
+                                            "zs_logprobs_backward", "zs_lmhead_logprobs",
+                                            "zs_lmhead_logprobs_workspace", "zs_embed",
+                                            "zs_embed_backward", "zs_embed_backward_workspace"):
             f.restype = C.c_int
     _lib = L
     return L

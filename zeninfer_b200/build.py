@@ -27,7 +27,8 @@ WORKLOAD_SO = os.path.join(HERE, "libzs_workload.so")
 HOST_API_BENCH = os.path.join(HERE, "bench_host_api")
 
 SAMPLER_SOURCES = ["zs_sampler.cu", "zs_noalloc_scratch.cu", "sample_shim.cpp"]
-SAMPLER_DEPS = SAMPLER_SOURCES + ["zs_kernels.cuh", "zs_device.cuh", "zs_stats.cuh", "zs_lmhead.cuh"]
+SAMPLER_DEPS = SAMPLER_SOURCES + ["zs_kernels.cuh", "zs_device.cuh", "zs_stats.cuh", "zs_lmhead.cuh",
+                                  "zs_logprobs.cuh", "zs_embed.cuh"]
 
 NVCC_ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = NVCC_ARCH + ["-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC",

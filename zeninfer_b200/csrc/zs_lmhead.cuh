@@ -37,6 +37,7 @@
 
 #include "zs_device.cuh"
 #include "zs_kernels.cuh"
+#include "zs_logprobs.cuh"
 
 namespace zs {
 
@@ -93,6 +94,11 @@ struct LmArgs {
     uint32_t* tau;               // optional [B] value orders shared by a row's slices
     int* status;
     int32_t pair;                // 2: zs_lmhead_kernel<2> (CTA pairs), else <1>; host only
+    // statistics instead of a shortlist (zs_lmhead_kernel<P, true>): per (row, slice)
+    // the maximum, sum of 2^t and sum of 2^t t of the slice's logits (LpStat)
+    float4* stats;               // [B][S]
+    float temp;
+    const float* row_temp;
 };
 
 // ---- PTX wrappers: TMA tiles and the 5th-generation tensor cores ----
@@ -760,12 +766,39 @@ __device__ __forceinline__ void lm_chunk(const uint32_t (&r)[16], int col0, int 
     }
 }
 
+// One 32-column chunk of a tile into the running statistics of this warp's 16 rows, each
+// row's columns split over a lane pair as in lm_chunk.  Columns beyond the vocabulary
+// count as -1e30: they never raise a maximum that a real column set, and 2^t is 0.
+__device__ __forceinline__ void lm_stat_chunk(const uint32_t (&r)[16], int col0, int par, int V,
+                                              float c, LpStat& st) {
+    float v[16];
+#pragma unroll
+    for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(r[j]);
+    if (col0 + 32 > V) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+            if (col0 + par + 2 * j >= V) v[j] = -1e30f;
+    }
+    float b[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) b[j] = fmaxf(v[j], v[j + 8]);
+#pragma unroll
+    for (int w = 4; w >= 1; w >>= 1)
+#pragma unroll
+        for (int j = 0; j < w; ++j) b[j] = fmaxf(b[j], b[j + w]);
+    if (b[0] > st.m) lp_raise(st, b[0], c);
+    const float base = st.m == -INFINITY ? 0.0f : st.m;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) lp_add(st, v[j], base, c);
+}
+
 // P = 1: one CTA per tile.  P = 2: launched in clusters of two CTAs, each pair one
 // 256 x 256 tile at a time (LmGeom); the leader (cluster rank 0) issues the MMAs for
 // both, the copies of both CTAs count on the leader's barriers, the MMA commits
 // arrive on both CTAs' barriers, and both epilogues free an accumulator on the
 // leader's barrier.
-template <int P>
+// STATS: the epilogue keeps each row's log-probability statistics instead of candidates.
+template <int P, bool STATS = false>
 __global__ void __launch_bounds__(kLmThreads, 1)
     zs_lmhead_kernel(const __grid_constant__ CUtensorMap tm_a,
                      const __grid_constant__ CUtensorMap tm_b,
@@ -978,7 +1011,10 @@ __global__ void __launch_bounds__(kLmThreads, 1)
             const int row = m * G::kRows + (int)rank * kLmM + r_in;
             const bool valid = row < a.B;
             uint32_t keff = 1;
-            if (valid) {
+            LpStat stat = lp_empty();
+            const float stat_c =
+                STATS && valid ? lp_inv_temp(a.temp, a.row_temp, row) * kLpLog2e : 1.0f;
+            if (!STATS && valid) {
                 const RowPlan rp = plan_row(load_params(a.row_params, a.shared, row), a.V_total,
                                             nullptr, nullptr, 0, row);
                 keff = (uint32_t)rp.ksel;
@@ -1021,6 +1057,10 @@ __global__ void __launch_bounds__(kLmThreads, 1)
                     for (int j = 0; j < 16; ++j) ra[j] = rb[j];
                     __syncwarp();
                     if (c + 1 < G::kCols / 32) tc_ld16_issue(base + (uint32_t)((c + 1) * 32), rb);
+                    if constexpr (STATS) {
+                        lm_stat_chunk(ra, tcol + c * 32, par, a.V, stat_c, stat);
+                        continue;
+                    }
                     if (a.tma_out) {
                         // logits only: this warp's 16 rows x 32 columns go to a staging
                         // buffer in the (here unused) candidate area, in the 128-byte
@@ -1064,6 +1104,16 @@ __global__ void __launch_bounds__(kLmThreads, 1)
                 }
             }
             if (!ok) break;
+            if constexpr (STATS) {
+                LpStat other;
+                other.m = __shfl_xor_sync(kFull, stat.m, 2);
+                other.s = __shfl_xor_sync(kFull, stat.s, 2);
+                other.w = __shfl_xor_sync(kFull, stat.w, 2);
+                stat = lp_merge(stat, other, stat_c);
+                if (valid && owner)
+                    a.stats[(int64_t)row * a.S + s] = make_float4(stat.m, stat.s, stat.w, 0.0f);
+                continue;
+            }
             if (!a.select) continue;
             // The run goes on into the next slice of this row tile: this slice's
             // block stays empty and the buffer carries over.
@@ -1104,6 +1154,65 @@ __global__ void __launch_bounds__(kLmThreads, 1)
             tc_dealloc(tmem, kLmTmemCols);
         else
             tc_dealloc_pair(tmem, kLmTmemCols);
+    }
+}
+
+// Joins a row's slices (zs_lmhead_kernel<P, true>) and takes the given ids' logits as
+// f32 dot products of xn and the id's weight row (bf16 products are exact in f32): one
+// warp per row.
+struct LmLogprobArgs {
+    const float4* stats;
+    int32_t B, E, V, S;
+    const __nv_bfloat16* xn;
+    const __nv_bfloat16* w;
+    float temp;
+    const float* row_temp;
+    const int32_t* ids;
+    int64_t ids_ld;
+    int32_t n_ids;
+    float* out_logp;
+    float* out_entropy;
+    float* out_lse;
+};
+constexpr int kLmLogprobWarps = 4;
+__global__ void __launch_bounds__(32 * kLmLogprobWarps) zs_lm_logprob_kernel(const LmLogprobArgs a) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int64_t row = (int64_t)blockIdx.x * kLmLogprobWarps + warp;
+    if (row >= a.B) return;
+    const float it = lp_inv_temp(a.temp, a.row_temp, row);
+    const float c = it * kLpLog2e;
+    LpStat st = lp_empty();
+    for (int s = lane; s < a.S; s += 32) {
+        const float4 q = a.stats[row * a.S + s];
+        st = lp_merge(st, {q.x, q.y, q.z}, c);
+    }
+    st = lp_warp_merge(st, c);
+    const double log_s = st.s == 0.0f ? -INFINITY : log((double)st.s);
+    const uint4* xr = reinterpret_cast<const uint4*>(a.xn + row * a.E);
+    for (int j = 0; j < a.n_ids; ++j) {
+        const int32_t id = a.ids[row * a.ids_ld + j];
+        float lp = 0.0f;
+        if (id >= 0 && id < a.V) {
+            const uint4* wr = reinterpret_cast<const uint4*>(a.w + (int64_t)id * a.E);
+            float dot = 0.0f;
+            for (int i = lane; i < a.E / 8; i += 32) {
+                float xv[8], wv[8];
+                lp_unpack(xr[i], xv, __nv_bfloat16());
+                lp_unpack(__ldg(wr + i), wv, __nv_bfloat16());
+#pragma unroll
+                for (int e = 0; e < 8; ++e) dot = fmaf(xv[e], wv[e], dot);
+            }
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) dot += __shfl_xor_sync(kFull, dot, o);
+            lp = lp_value(dot, st.m, log_s, it);
+            if (lp > 0.0f) lp = 0.0f;  // the two summation orders differ by their roundings
+        }
+        if (lane == 0) a.out_logp[row * a.n_ids + j] = lp;
+    }
+    if (lane == 0) {
+        if (a.out_entropy) a.out_entropy[row] = lp_entropy(st, log_s);
+        if (a.out_lse)
+            a.out_lse[row] = st.s == 0.0f ? -INFINITY : (float)((double)st.m * (double)it + log_s);
     }
 }
 

@@ -23,8 +23,10 @@
 #include <cudaTypedefs.h>
 #include <nvtx3/nvToolsExt.h>
 
+#include "zs_embed.cuh"
 #include "zs_kernels.cuh"
 #include "zs_lmhead.cuh"
+#include "zs_logprobs.cuh"
 #include "zs_sampler.h"
 #include "zs_stats.cuh"
 
@@ -41,6 +43,10 @@ struct NvtxRange {
 static_assert(sizeof(zs_params) == sizeof(zs::Params), "zs_params layout");
 static_assert(sizeof(zs_row_info) == sizeof(zs::RowInfo), "zs_row_info layout");
 static_assert(sizeof(zs_row_info) == 48, "zs_row_info size");
+static_assert(sizeof(zs_logprob_row) == sizeof(zs::LpRow) && sizeof(zs_logprob_row) == 16,
+              "zs_logprob_row layout");
+static_assert(ZS_LOGPROBS_MAX_TOP == zs::kLpMaxTop && ZS_LOGPROBS_MAX_IDS == zs::kLpMaxIds,
+              "log-probability limits");
 
 namespace {
 
@@ -357,7 +363,7 @@ struct zs_context {
     size_t fail_units_n = 0;
     // optional per-kernel timing (zs_set_timing): event pairs around each launch
     struct TimedLaunch {
-        int kind;  // 0 select, 1 merge, 2 large, 3 lm_head GEMM, 4 lm_head rmsnorm
+        int kind;  // 0 select, 1 merge, 2 large, 3 lm_head GEMM, 4 lm_head rmsnorm; -1: counted only
         cudaEvent_t begin, end;
     };
     bool timing = false;
@@ -365,6 +371,7 @@ struct zs_context {
     int32_t lm_tiles = ZS_LMHEAD_TILES_AUTO;  // zs_set_lmhead_tiles
     int lm_pairs = 0;                         // resident CTA pairs of zs_lmhead_kernel<2>
     int32_t spec_mode = ZS_SPECULATION_ON;    // zs_set_speculation
+    int lp_max_cl = 8;                        // CTAs per row of zs_logprobs_kernel at most
     int small_clusters = 0;                   // zs_small_kernel clusters resident at once (0: none)
     int32_t small_max_rows = 8;               // zs_set_small_batch
     std::vector<TimedLaunch> timed;      // recorded since the last zs_get_timing
@@ -459,7 +466,7 @@ struct LaunchScope {
     cudaEvent_t b = nullptr, e = nullptr;
     LaunchScope(zs_context* h_, int kind_, cudaStream_t st_) : h(h_), kind(kind_), st(st_) {
         h->launches += 1;
-        if (!h->timing) return;
+        if (!h->timing || kind < 0) return;
         b = take();
         e = take();
         if (b && e) cudaEventRecord(b, st);
@@ -810,6 +817,235 @@ zs_status wait_collectives(zs_context* h, void* comm, cudaStream_t st, Clock::ti
 
 }  // namespace
 
+// ---- log probabilities and the embedding table: launches ----
+namespace {
+
+template <typename T, int NT, bool TOP>
+cudaError_t setup_logprobs(int* max_cl) {
+    auto k = zs::zs_logprobs_kernel<T, NT, TOP>;
+    cudaError_t e = cudaSuccess;
+    if (TOP)
+        e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 (int)sizeof(zs::LpTopSmem<NT>));
+    if (e != cudaSuccess) return e;
+    // 16 CTAs per row is a non-portable cluster size; where it is refused or cannot be
+    // resident, 8 are used
+    bool ok = cudaFuncSetAttribute(k, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess;
+    if (ok) {
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = zs::kLpMaxCl;
+        attr[0].val.clusterDim.y = 1;
+        attr[0].val.clusterDim.z = 1;
+        cudaLaunchConfig_t cfg;
+        std::memset(&cfg, 0, sizeof(cfg));
+        cfg.gridDim = dim3(zs::kLpMaxCl);
+        cfg.blockDim = dim3(NT);
+        cfg.dynamicSmemBytes = TOP ? sizeof(zs::LpTopSmem<NT>) : 0;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        int n = 0;
+        ok = cudaOccupancyMaxActiveClusters(&n, k, &cfg) == cudaSuccess && n > 0;
+    }
+    (void)cudaGetLastError();
+    if (!ok) *max_cl = std::min(*max_cl, 8);
+    return cudaSuccess;
+}
+
+template <typename T>
+cudaError_t setup_logprobs_type(int* max_cl) {
+    cudaError_t e = setup_logprobs<T, 256, true>(max_cl);
+    if (e == cudaSuccess) e = setup_logprobs<T, 256, false>(max_cl);
+    if (e == cudaSuccess) e = setup_logprobs<T, 1024, true>(max_cl);
+    if (e == cudaSuccess) e = setup_logprobs<T, 1024, false>(max_cl);
+    return e;
+}
+
+cudaError_t setup_vocab_ops(int* max_cl) {
+    *max_cl = zs::kLpMaxCl;
+    cudaError_t e = setup_logprobs_type<float>(max_cl);
+    if (e == cudaSuccess) e = setup_logprobs_type<__half>(max_cl);
+    if (e == cudaSuccess) e = setup_logprobs_type<__nv_bfloat16>(max_cl);
+    if (e == cudaSuccess)
+        e = cudaFuncSetAttribute(zs::zs_embed_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 (int)sizeof(zs::EsSmem));
+    return e;
+}
+
+int dtype_size(int32_t dtype) {
+    return dtype == ZS_DTYPE_F32 ? 4 : (dtype == ZS_DTYPE_F16 || dtype == ZS_DTYPE_BF16) ? 2 : 0;
+}
+
+bool misaligned(const void* p, uintptr_t a) { return ((uintptr_t)p & (a - 1)) != 0; }
+
+// CTAs per row of zs_logprobs_kernel, and the threads of each.
+struct LpShape {
+    int cl, nt;
+};
+LpShape lp_shape(const zs_context* h, int64_t batch, int64_t n, int esize) {
+    const int64_t vecs = n * esize / 16;
+    LpShape s;
+    if (batch * zs::kLpMaxCl <= h->num_sms && vecs >= 4096) {
+        s.nt = 1024;
+        s.cl = h->lp_max_cl;
+    } else {
+        s.nt = 256;
+        s.cl = 1;
+        while (s.cl < h->lp_max_cl && batch * s.cl < (int64_t)h->num_sms * 8 && vecs / (2 * s.cl) >= 512)
+            s.cl *= 2;
+    }
+    return s;
+}
+
+template <typename T, int NT, bool TOP>
+zs_status launch_logprobs(zs_context* h, const zs::LpArgs& a, cudaStream_t st) {
+    LaunchScope scope(h, -1, st);
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)a.cl;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg;
+    std::memset(&cfg, 0, sizeof(cfg));
+    cfg.gridDim = dim3((unsigned)((int64_t)a.B * a.cl));
+    cfg.blockDim = dim3(NT);
+    cfg.dynamicSmemBytes = TOP ? sizeof(zs::LpTopSmem<NT>) : 0;
+    cfg.stream = st;
+    cfg.attrs = attr;
+    cfg.numAttrs = a.cl > 1 ? 1 : 0;
+    ZS_CUDA(cudaLaunchKernelEx(&cfg, zs::zs_logprobs_kernel<T, NT, TOP>, a));
+    return ZS_OK;
+}
+
+template <typename T>
+zs_status launch_logprobs_type(zs_context* h, const zs::LpArgs& a, int nt, cudaStream_t st) {
+    if (nt == 256)
+        return a.k > 0 ? launch_logprobs<T, 256, true>(h, a, st) : launch_logprobs<T, 256, false>(h, a, st);
+    return a.k > 0 ? launch_logprobs<T, 1024, true>(h, a, st) : launch_logprobs<T, 1024, false>(h, a, st);
+}
+
+// Checks shared by zs_logprobs and its backward pass.
+zs_status lp_validate(zs_handle h, const void* logits, int32_t dtype, int64_t ld, int32_t batch,
+                      int32_t n_vocab, const int32_t* ids, int64_t ids_ld, int32_t n_ids) {
+    if (!h) return fail(ZS_ERR_INVALID_ARGUMENT, "null handle");
+    if (batch < 0) return fail(ZS_ERR_INVALID_ARGUMENT, "batch < 0");
+    const int es = dtype_size(dtype);
+    if (es == 0) return fail(ZS_ERR_INVALID_ARGUMENT, "unknown dtype");
+    if (n_ids < 0 || n_ids > ZS_LOGPROBS_MAX_IDS)
+        return fail(ZS_ERR_INVALID_ARGUMENT, "n_ids must be 0 to ZS_LOGPROBS_MAX_IDS");
+    if (batch == 0) return ZS_OK;
+    if (n_vocab < 1) return fail(ZS_ERR_INVALID_ARGUMENT, "n_vocab < 1");
+    if (!logits) return fail(ZS_ERR_INVALID_ARGUMENT, "logits is null");
+    if (misaligned(logits, es)) return fail(ZS_ERR_INVALID_ARGUMENT, "logits not aligned to its type");
+    if (ld < n_vocab) return fail(ZS_ERR_INVALID_ARGUMENT, "ld < n_vocab");
+    if (batch > 1 && ld > (int64_t)1 << 40) return fail(ZS_ERR_INVALID_ARGUMENT, "ld too large");
+    if (n_ids > 0) {
+        if (!ids || misaligned(ids, 4)) return fail(ZS_ERR_INVALID_ARGUMENT, "ids is null or misaligned");
+        if (ids_ld < n_ids) return fail(ZS_ERR_INVALID_ARGUMENT, "ids_ld < n_ids");
+        if (batch > 1 && ids_ld > (int64_t)1 << 40) return fail(ZS_ERR_INVALID_ARGUMENT, "ids_ld too large");
+    }
+    return ZS_OK;
+}
+
+template <typename T>
+cudaError_t launch_lp_backward(const zs::LpBackArgs& base, cudaStream_t st) {
+    zs::LpBackArgs a = base;
+    a.chunks = (int32_t)(((int64_t)a.n + zs::lp_back_chunk<T>() - 1) / zs::lp_back_chunk<T>());
+    zs::zs_logprobs_backward_kernel<T>
+        <<<(unsigned)((int64_t)a.B * a.chunks), zs::kLpBackThreads, 0, st>>>(a);
+    return cudaGetLastError();
+}
+
+template <typename TI, typename TO, bool VEC>
+cudaError_t launch_embed(const zs_context* h, zs::EmArgs a, cudaStream_t st) {
+    constexpr int G = VEC ? zs::EmGran<TI, TO>::G : 1;
+    const int gran = std::max(1, a.E / G);
+    a.tpr = 32;
+    while (a.tpr < zs::kEmThreads && a.tpr < gran) a.tpr *= 2;
+    const int at_once = zs::kEmThreads / a.tpr;
+    // four rows per thread once that still gives every SM several CTAs
+    if (a.n >= (int64_t)h->num_sms * 8 * at_once * 4) {
+        const int64_t grid = (a.n + at_once * 4 - 1) / (at_once * 4);
+        zs::zs_embed_kernel<TI, TO, 4, VEC><<<(unsigned)grid, zs::kEmThreads, 0, st>>>(a);
+    } else {
+        const int64_t grid = (a.n + at_once - 1) / at_once;
+        zs::zs_embed_kernel<TI, TO, 1, VEC><<<(unsigned)grid, zs::kEmThreads, 0, st>>>(a);
+    }
+    return cudaGetLastError();
+}
+template <typename TI, typename TO>
+cudaError_t launch_embed_vec(const zs_context* h, const zs::EmArgs& a, cudaStream_t st) {
+    const bool vec = !misaligned(a.table, 16) && !misaligned(a.out, 16) &&
+                     a.table_ld * (int64_t)sizeof(TI) % 16 == 0 &&
+                     a.out_ld * (int64_t)sizeof(TO) % 16 == 0;
+    return vec ? launch_embed<TI, TO, true>(h, a, st) : launch_embed<TI, TO, false>(h, a, st);
+}
+template <typename TI>
+cudaError_t launch_embed_in(const zs_context* h, const zs::EmArgs& a, int32_t out_dtype, cudaStream_t st) {
+    if (out_dtype == ZS_DTYPE_F32) return launch_embed_vec<TI, float>(h, a, st);
+    if (out_dtype == ZS_DTYPE_F16) return launch_embed_vec<TI, __half>(h, a, st);
+    return launch_embed_vec<TI, __nv_bfloat16>(h, a, st);
+}
+
+// Where the pairs and partial sums of zs_embed_backward lie in its workspace.
+struct EmbedWs {
+    int64_t pair_bytes, part_at, total;
+    int chunks;
+};
+EmbedWs embed_ws(int64_t n, int64_t E) {
+    EmbedWs w;
+    w.chunks = (int)((n + zs::kEsChunk - 1) / zs::kEsChunk);
+    w.pair_bytes = (n * 4 + 255) / 256 * 256;
+    w.part_at = 4 * w.pair_bytes;
+    w.total = w.part_at + ((int64_t)w.chunks * 2 * E * 4 + 255) / 256 * 256;
+    return w;
+}
+
+template <typename TG, typename TT, bool VEC>
+zs_status launch_embed_sum(zs_context* h, const zs::EbArgs& a, cudaStream_t st) {
+    constexpr int G = VEC ? zs::EmGran<TG, TT>::G : 1;
+    const int gran = (a.E + G - 1) / G;
+    const int bx = std::min(128, (gran + 31) / 32 * 32);
+    const unsigned tiles = (unsigned)((gran + bx - 1) / bx);
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg;
+    std::memset(&cfg, 0, sizeof(cfg));
+    cfg.stream = st;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    {
+        LaunchScope scope(h, -1, st);
+        cfg.gridDim = dim3((unsigned)a.chunks, tiles);
+        cfg.blockDim = dim3(bx);
+        ZS_CUDA(cudaLaunchKernelEx(&cfg, zs::zs_embed_sum_kernel<TG, TT, VEC>, a));
+    }
+    if (a.chunks > 1) {
+        LaunchScope scope(h, -1, st);
+        cfg.gridDim = dim3((unsigned)std::min(a.chunks - 1, h->num_sms), tiles);
+        cfg.blockDim = dim3(bx, zs::kEjGroups);
+        cfg.dynamicSmemBytes = (size_t)bx * zs::kEjGroups * G * sizeof(float);
+        ZS_CUDA(cudaLaunchKernelEx(&cfg, zs::zs_embed_join_kernel<TG, TT, VEC>, a));
+    }
+    return ZS_OK;
+}
+template <typename TG, typename TT>
+zs_status launch_embed_sum_vec(zs_context* h, const zs::EbArgs& a, cudaStream_t st) {
+    const bool vec = a.E % zs::EmGran<TG, TT>::G == 0 && !misaligned(a.grad, 16) &&
+                     !misaligned(a.table, 16) && a.grad_ld * (int64_t)sizeof(TG) % 16 == 0 &&
+                     a.table_ld * (int64_t)sizeof(TT) % 16 == 0;
+    return vec ? launch_embed_sum<TG, TT, true>(h, a, st) : launch_embed_sum<TG, TT, false>(h, a, st);
+}
+template <typename TG>
+zs_status launch_embed_sum_in(zs_context* h, const zs::EbArgs& a, int32_t table_dtype, cudaStream_t st) {
+    if (table_dtype == ZS_DTYPE_F32) return launch_embed_sum_vec<TG, float>(h, a, st);
+    if (table_dtype == ZS_DTYPE_F16) return launch_embed_sum_vec<TG, __half>(h, a, st);
+    return launch_embed_sum_vec<TG, __nv_bfloat16>(h, a, st);
+}
+
+}  // namespace
+
 extern "C" {
 
 int zs_abi_version(void) { return ZS_ABI_VERSION; }
@@ -873,6 +1109,14 @@ zs_status zs_create(int device, zs_handle* out) {
         (e = cudaFuncSetAttribute(zs::zs_lm_exact_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                   (int)zs::ex_smem_bytes(1, zs::kExMaxElems))) != cudaSuccess)
         return cleanup(cuda_fail(e, "cudaFuncSetAttribute zs_lm_exact_kernel"));
+    if ((size_t)prop.sharedMemPerBlockOptin >= zs::kLmSmemBytes &&
+        ((e = cudaFuncSetAttribute(zs::zs_lmhead_kernel<1, true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                   (int)zs::kLmSmemBytes)) != cudaSuccess ||
+         (e = cudaFuncSetAttribute(zs::zs_lmhead_kernel<2, true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                   (int)zs::kLmSmemBytes)) != cudaSuccess))
+        return cleanup(cuda_fail(e, "cudaFuncSetAttribute zs_lmhead_kernel (statistics)"));
+    if ((e = setup_vocab_ops(&h->lp_max_cl)) != cudaSuccess)
+        return cleanup(cuda_fail(e, "cudaFuncSetAttribute (log probabilities, embedding)"));
     // CTA pairs of the lm_head kernel that can be resident at once (0: none; the
     // one-CTA tiles are used then).
     h->lm_pairs = 0;
@@ -1241,12 +1485,19 @@ zs_status lm_validate(zs_handle h, const float* hidden, int64_t hidden_ld, const
 
 // rmsnorm into the handle's bf16 rows, then zs_lmhead_kernel over `a` (whose B, E,
 // V, S, select, parameters and outputs the caller has set).
+// xn: where the normalised rows go ([B][E] bf16, 16-byte aligned), or null for handle
+// scratch.
 zs_status lm_run(zs_context* h, const float* hidden, int64_t hidden_ld, const float* norm_w,
-                 float eps, const void* weight, zs::LmArgs& a, cudaStream_t st) {
-    zs_status s = grow((void**)&h->lm_xn, &h->lm_xn_bytes, (size_t)a.B * a.E * 2);
-    if (s != ZS_OK) return s;
+                 float eps, const void* weight, zs::LmArgs& a, cudaStream_t st,
+                 void* xn = nullptr) {
+    zs_status s = ZS_OK;
+    if (!xn) {
+        s = grow((void**)&h->lm_xn, &h->lm_xn_bytes, (size_t)a.B * a.E * 2);
+        if (s != ZS_OK) return s;
+        xn = h->lm_xn;
+    }
     CUtensorMap tm_a, tm_b, tm_c;
-    s = lm_tensor_map(h, &tm_a, h->lm_xn, a.B, a.E);
+    s = lm_tensor_map(h, &tm_a, xn, a.B, a.E);
     if (s == ZS_OK) s = lm_tensor_map(h, &tm_b, weight, a.V, a.E);
     if (s != ZS_OK) return s;
     // logits only: the epilogue stores 32 x 32 tiles by TMA (its candidate buffers
@@ -1283,7 +1534,7 @@ zs_status lm_run(zs_context* h, const float* hidden, int64_t hidden_ld, const fl
         const size_t smem = (size_t)nw * a.E * sizeof(float);
         const int grid = (int)std::min<int64_t>((a.B + nw - 1) / nw, (int64_t)h->num_sms * 16);
         zs::zs_lm_rmsnorm_kernel<<<grid, nw * 32, smem, st>>>(
-            hidden, hidden_ld, norm_w, eps, a.B, a.E, reinterpret_cast<__nv_bfloat16*>(h->lm_xn),
+            hidden, hidden_ld, norm_w, eps, a.B, a.E, reinterpret_cast<__nv_bfloat16*>(xn),
             a.tau);
         ZS_CUDA(cudaGetLastError());
     }
@@ -1310,7 +1561,11 @@ zs_status lm_run(zs_context* h, const float* hidden, int64_t hidden_ld, const fl
         cfg.stream = st;
         cfg.attrs = attr;
         cfg.numAttrs = a.pair == 2 ? 2 : 1;
-        if (a.pair == 2)
+        if (a.stats)
+            ZS_CUDA(a.pair == 2
+                        ? cudaLaunchKernelEx(&cfg, zs::zs_lmhead_kernel<2, true>, tm_a, tm_b, tm_c, a)
+                        : cudaLaunchKernelEx(&cfg, zs::zs_lmhead_kernel<1, true>, tm_a, tm_b, tm_c, a));
+        else if (a.pair == 2)
             ZS_CUDA(cudaLaunchKernelEx(&cfg, zs::zs_lmhead_kernel<2>, tm_a, tm_b, tm_c, a));
         else
             ZS_CUDA(cudaLaunchKernelEx(&cfg, zs::zs_lmhead_kernel<1>, tm_a, tm_b, tm_c, a));
@@ -1609,6 +1864,333 @@ zs_status zs_logits_stats(zs_handle h, const float* logits, int64_t ld, int32_t 
     zs::zs_stats_final_kernel<<<std::min(batch, 65535), 32, 0, st>>>(a);
     ZS_CUDA(cudaGetLastError());
     return ZS_OK;
+}
+
+zs_status zs_logprobs(zs_handle h, const void* logits, int32_t dtype, int64_t ld, int32_t batch,
+                      int32_t n_vocab, float temp, const float* row_temp, const int32_t* ids,
+                      int64_t ids_ld, int32_t n_ids, float* out_logp, int32_t topn,
+                      int32_t* top_ids, float* top_logp, float* out_entropy, float* out_lse,
+                      zs_logprob_row* out_rows, void* stream) {
+    NvtxRange nvtx_range("zs_logprobs");
+    zs_status s = lp_validate(h, logits, dtype, ld, batch, n_vocab, ids, ids_ld, n_ids);
+    if (s != ZS_OK) return s;
+    if (topn < 0 || topn > ZS_LOGPROBS_MAX_TOP)
+        return fail(ZS_ERR_INVALID_ARGUMENT, "topn must be 0 to ZS_LOGPROBS_MAX_TOP");
+    if (temp != temp) return fail(ZS_ERR_INVALID_ARGUMENT, "temp is NaN");
+    if (batch == 0) return ZS_OK;
+    if (n_ids > 0 && !out_logp) return fail(ZS_ERR_INVALID_ARGUMENT, "out_logp is null");
+    if (topn > 0 && (!top_ids || !top_logp))
+        return fail(ZS_ERR_INVALID_ARGUMENT, "top_ids or top_logp is null");
+    if (misaligned(row_temp, 4) || misaligned(out_logp, 4) || misaligned(top_ids, 4) ||
+        misaligned(top_logp, 4) || misaligned(out_entropy, 4) || misaligned(out_lse, 4) ||
+        misaligned(out_rows, 16))
+        return fail(ZS_ERR_INVALID_ARGUMENT, "a misaligned output (4 bytes; out_rows 16)");
+    DeviceGuard g(h->device);
+    if (!g.ok) return fail(ZS_ERR_CUDA, "cudaSetDevice failed");
+    zs::LpArgs a;
+    std::memset(&a, 0, sizeof(a));
+    a.logits = logits;
+    a.ld = ld;
+    a.B = batch;
+    a.n = n_vocab;
+    a.temp = temp;
+    a.row_temp = row_temp;
+    a.ids = ids;
+    a.ids_ld = ids_ld;
+    a.n_ids = n_ids;
+    a.k = std::min(topn, n_vocab);
+    a.top_ld = topn;
+    a.out_logp = out_logp;
+    a.top_ids = top_ids;
+    a.top_logp = top_logp;
+    a.out_entropy = out_entropy;
+    a.out_lse = out_lse;
+    a.out_rows = reinterpret_cast<zs::LpRow*>(out_rows);
+    const LpShape shape = lp_shape(h, batch, n_vocab, dtype_size(dtype));
+    a.cl = shape.cl;
+    cudaStream_t st = (cudaStream_t)stream;
+    if (dtype == ZS_DTYPE_F32) return launch_logprobs_type<float>(h, a, shape.nt, st);
+    if (dtype == ZS_DTYPE_F16) return launch_logprobs_type<__half>(h, a, shape.nt, st);
+    return launch_logprobs_type<__nv_bfloat16>(h, a, shape.nt, st);
+}
+
+zs_status zs_logprobs_backward(zs_handle h, const void* logits, int32_t dtype, int64_t ld,
+                               int32_t batch, int32_t n_vocab, const zs_logprob_row* rows,
+                               const int32_t* ids, int64_t ids_ld, int32_t n_ids,
+                               const float* grad_logp, const float* grad_entropy,
+                               const float* grad_lse, void* grad_logits, int64_t grad_ld,
+                               void* stream) {
+    NvtxRange nvtx_range("zs_logprobs_backward");
+    zs_status s = lp_validate(h, logits, dtype, ld, batch, n_vocab, ids, ids_ld, n_ids);
+    if (s != ZS_OK) return s;
+    if (batch == 0) return ZS_OK;
+    if (!rows || misaligned(rows, 16))
+        return fail(ZS_ERR_INVALID_ARGUMENT, "rows is null or not 16-byte aligned");
+    if (n_ids > 0 && !grad_logp)
+        return fail(ZS_ERR_INVALID_ARGUMENT, "ids without grad_logp");
+    if (misaligned(grad_logp, 4) || misaligned(grad_entropy, 4) || misaligned(grad_lse, 4))
+        return fail(ZS_ERR_INVALID_ARGUMENT, "a gradient is not 4-byte aligned");
+    if (!grad_logits || misaligned(grad_logits, dtype_size(dtype)))
+        return fail(ZS_ERR_INVALID_ARGUMENT, "grad_logits is null or not aligned to its type");
+    if (grad_ld < n_vocab) return fail(ZS_ERR_INVALID_ARGUMENT, "grad_ld < n_vocab");
+    if (batch > 1 && grad_ld > (int64_t)1 << 40)
+        return fail(ZS_ERR_INVALID_ARGUMENT, "grad_ld too large");
+    if ((int64_t)batch * (n_vocab / zs::lp_back_chunk<float>() + 1) > 0x7fffffff)
+        return fail(ZS_ERR_INVALID_ARGUMENT, "batch x n_vocab too large for one call");
+    if (grad_logits == logits && grad_ld != ld && batch > 1)
+        return fail(ZS_ERR_INVALID_ARGUMENT, "in place, grad_ld must equal ld");
+    DeviceGuard g(h->device);
+    if (!g.ok) return fail(ZS_ERR_CUDA, "cudaSetDevice failed");
+    zs::LpBackArgs a;
+    std::memset(&a, 0, sizeof(a));
+    a.logits = logits;
+    a.ld = ld;
+    a.B = batch;
+    a.n = n_vocab;
+    a.rows = reinterpret_cast<const zs::LpRow*>(rows);
+    a.ids = ids;
+    a.ids_ld = ids_ld;
+    a.n_ids = n_ids;
+    a.g_logp = n_ids > 0 ? grad_logp : nullptr;
+    a.g_entropy = grad_entropy;
+    a.g_lse = grad_lse;
+    a.grad = grad_logits;
+    a.grad_ld = grad_ld;
+    cudaStream_t st = (cudaStream_t)stream;
+    LaunchScope scope(h, -1, st);
+    ZS_CUDA(dtype == ZS_DTYPE_F32   ? launch_lp_backward<float>(a, st)
+            : dtype == ZS_DTYPE_F16 ? launch_lp_backward<__half>(a, st)
+                                    : launch_lp_backward<__nv_bfloat16>(a, st));
+    return ZS_OK;
+}
+
+zs_status zs_lmhead_logprobs_workspace(zs_handle h, int32_t batch, int32_t n_embd, int32_t n_vocab,
+                                       int64_t* out_bytes) {
+    if (!h || !out_bytes) return fail(ZS_ERR_INVALID_ARGUMENT, "null handle or out_bytes");
+    if (batch < 0 || n_embd < 1 || n_vocab < 1)
+        return fail(ZS_ERR_INVALID_ARGUMENT, "batch < 0, n_embd < 1 or n_vocab < 1");
+    zs::LmArgs a;
+    std::memset(&a, 0, sizeof(a));
+    if (batch > 0) lm_geometry(h, a, batch, n_vocab, 1024);
+    *out_bytes = ((int64_t)batch * n_embd * 2 + 255) / 256 * 256 + (int64_t)batch * a.S * 16;
+    return ZS_OK;
+}
+
+zs_status zs_lmhead_logprobs(zs_handle h, const float* hidden, int64_t hidden_ld,
+                             const float* norm_w, float eps, const void* weight, int32_t batch,
+                             int32_t n_embd, int32_t n_vocab, float temp, const float* row_temp,
+                             const int32_t* ids, int64_t ids_ld, int32_t n_ids, float* out_logp,
+                             float* out_entropy, float* out_lse, void* workspace,
+                             int64_t workspace_bytes, void* stream) {
+    NvtxRange nvtx_range("zs_lmhead_logprobs");
+    if (!h) return fail(ZS_ERR_INVALID_ARGUMENT, "null handle");
+    if (batch < 0) return fail(ZS_ERR_INVALID_ARGUMENT, "batch < 0");
+    if (n_ids < 0 || n_ids > ZS_LOGPROBS_MAX_IDS)
+        return fail(ZS_ERR_INVALID_ARGUMENT, "n_ids must be 0 to ZS_LOGPROBS_MAX_IDS");
+    if (temp != temp) return fail(ZS_ERR_INVALID_ARGUMENT, "temp is NaN");
+    if (batch == 0) return ZS_OK;
+    zs_status s = lm_validate(h, hidden, hidden_ld, norm_w, weight, n_embd, n_vocab, nullptr, 0);
+    if (s != ZS_OK) return s;
+    if (n_ids > 0) {
+        if (!ids || misaligned(ids, 4) || !out_logp)
+            return fail(ZS_ERR_INVALID_ARGUMENT, "ids or out_logp is null or misaligned");
+        if (ids_ld < n_ids) return fail(ZS_ERR_INVALID_ARGUMENT, "ids_ld < n_ids");
+    }
+    if (misaligned(row_temp, 4) || misaligned(out_logp, 4) || misaligned(out_entropy, 4) ||
+        misaligned(out_lse, 4))
+        return fail(ZS_ERR_INVALID_ARGUMENT, "a misaligned array (4 bytes)");
+    int64_t need = 0;
+    s = zs_lmhead_logprobs_workspace(h, batch, n_embd, n_vocab, &need);
+    if (s != ZS_OK) return s;
+    if (!workspace || misaligned(workspace, 256) || workspace_bytes < need)
+        return fail(ZS_ERR_INVALID_ARGUMENT,
+                    "workspace is null, not 256-byte aligned or smaller than "
+                    "zs_lmhead_logprobs_workspace says");
+    DeviceGuard g(h->device);
+    if (!g.ok) return fail(ZS_ERR_CUDA, "cudaSetDevice failed");
+    cudaStream_t st = (cudaStream_t)stream;
+    uint8_t* ws = reinterpret_cast<uint8_t*>(workspace);
+    zs::LmArgs a;
+    std::memset(&a, 0, sizeof(a));
+    a.B = batch;
+    a.E = n_embd;
+    a.V = n_vocab;
+    a.V_total = n_vocab;
+    lm_geometry(h, a, batch, n_vocab, 1024);
+    a.stats = reinterpret_cast<float4*>(ws + ((int64_t)batch * n_embd * 2 + 255) / 256 * 256);
+    a.temp = temp;
+    a.row_temp = row_temp;
+    s = lm_run(h, hidden, hidden_ld, norm_w, eps, weight, a, st, ws);
+    if (s != ZS_OK) return s;
+    zs::LmLogprobArgs f;
+    std::memset(&f, 0, sizeof(f));
+    f.stats = a.stats;
+    f.B = batch;
+    f.E = n_embd;
+    f.V = n_vocab;
+    f.S = a.S;
+    f.xn = reinterpret_cast<const __nv_bfloat16*>(ws);
+    f.w = reinterpret_cast<const __nv_bfloat16*>(weight);
+    f.temp = temp;
+    f.row_temp = row_temp;
+    f.ids = ids;
+    f.ids_ld = ids_ld;
+    f.n_ids = n_ids;
+    f.out_logp = out_logp;
+    f.out_entropy = out_entropy;
+    f.out_lse = out_lse;
+    LaunchScope scope(h, -1, st);
+    zs::zs_lm_logprob_kernel<<<(batch + zs::kLmLogprobWarps - 1) / zs::kLmLogprobWarps,
+                               32 * zs::kLmLogprobWarps, 0, st>>>(f);
+    ZS_CUDA(cudaGetLastError());
+    return ZS_OK;
+}
+
+zs_status zs_embed(zs_handle h, const void* table, int32_t table_dtype, int64_t table_ld,
+                   int32_t n_vocab, int32_t n_embd, const int32_t* ids, int64_t n_tokens,
+                   float scale, void* out, int32_t out_dtype, int64_t out_ld, void* stream) {
+    NvtxRange nvtx_range("zs_embed");
+    if (!h) return fail(ZS_ERR_INVALID_ARGUMENT, "null handle");
+    const int ts = dtype_size(table_dtype), os = dtype_size(out_dtype);
+    if (ts == 0 || os == 0) return fail(ZS_ERR_INVALID_ARGUMENT, "unknown dtype");
+    if (n_tokens < 0 || n_tokens > ZS_EMBED_MAX_TOKENS)
+        return fail(ZS_ERR_INVALID_ARGUMENT, "n_tokens must be 0 to ZS_EMBED_MAX_TOKENS");
+    if (n_vocab < 1) return fail(ZS_ERR_INVALID_ARGUMENT, "n_vocab < 1");
+    if (n_embd < 1 || n_embd > ZS_EMBED_MAX_EMBD)
+        return fail(ZS_ERR_INVALID_ARGUMENT, "n_embd must be 1 to ZS_EMBED_MAX_EMBD");
+    if (n_tokens == 0) return ZS_OK;
+    if (!table || !ids || !out) return fail(ZS_ERR_INVALID_ARGUMENT, "table, ids or out is null");
+    if (misaligned(table, ts) || misaligned(out, os) || misaligned(ids, 4))
+        return fail(ZS_ERR_INVALID_ARGUMENT, "table, ids or out not aligned to its type");
+    if (table_ld < n_embd || out_ld < n_embd)
+        return fail(ZS_ERR_INVALID_ARGUMENT, "table_ld or out_ld < n_embd");
+    if (table_ld > (int64_t)1 << 30 || out_ld > (int64_t)1 << 30)
+        return fail(ZS_ERR_INVALID_ARGUMENT, "table_ld or out_ld too large");
+    DeviceGuard g(h->device);
+    if (!g.ok) return fail(ZS_ERR_CUDA, "cudaSetDevice failed");
+    zs::EmArgs a;
+    std::memset(&a, 0, sizeof(a));
+    a.table = table;
+    a.table_ld = table_ld;
+    a.V = n_vocab;
+    a.E = n_embd;
+    a.ids = ids;
+    a.n = n_tokens;
+    a.scale = scale;
+    a.out = out;
+    a.out_ld = out_ld;
+    cudaStream_t st = (cudaStream_t)stream;
+    LaunchScope scope(h, -1, st);
+    ZS_CUDA(table_dtype == ZS_DTYPE_F32   ? launch_embed_in<float>(h, a, out_dtype, st)
+            : table_dtype == ZS_DTYPE_F16 ? launch_embed_in<__half>(h, a, out_dtype, st)
+                                          : launch_embed_in<__nv_bfloat16>(h, a, out_dtype, st));
+    return ZS_OK;
+}
+
+zs_status zs_embed_backward_workspace(int64_t n_tokens, int32_t n_embd, int64_t* out_bytes) {
+    if (!out_bytes) return fail(ZS_ERR_INVALID_ARGUMENT, "out_bytes is null");
+    if (n_tokens < 0 || n_tokens > ZS_EMBED_MAX_TOKENS || n_embd < 1 || n_embd > ZS_EMBED_MAX_EMBD)
+        return fail(ZS_ERR_INVALID_ARGUMENT,
+                    "n_tokens must be 0 to ZS_EMBED_MAX_TOKENS, n_embd 1 to ZS_EMBED_MAX_EMBD");
+    *out_bytes = embed_ws(n_tokens, n_embd).total;
+    return ZS_OK;
+}
+
+zs_status zs_embed_backward(zs_handle h, const void* grad_out, int32_t grad_dtype, int64_t grad_ld,
+                            const int32_t* ids, int64_t n_tokens, float scale, int32_t n_vocab,
+                            int32_t n_embd, void* grad_table, int32_t table_dtype,
+                            int64_t table_ld, int32_t accumulate, void* workspace,
+                            int64_t workspace_bytes, void* stream) {
+    NvtxRange nvtx_range("zs_embed_backward");
+    if (!h) return fail(ZS_ERR_INVALID_ARGUMENT, "null handle");
+    const int gs = dtype_size(grad_dtype), ts = dtype_size(table_dtype);
+    if (gs == 0 || ts == 0) return fail(ZS_ERR_INVALID_ARGUMENT, "unknown dtype");
+    if (n_tokens < 0 || n_tokens > ZS_EMBED_MAX_TOKENS)
+        return fail(ZS_ERR_INVALID_ARGUMENT, "n_tokens must be 0 to ZS_EMBED_MAX_TOKENS");
+    if (n_vocab < 1) return fail(ZS_ERR_INVALID_ARGUMENT, "n_vocab < 1");
+    if (n_embd < 1 || n_embd > ZS_EMBED_MAX_EMBD)
+        return fail(ZS_ERR_INVALID_ARGUMENT, "n_embd must be 1 to ZS_EMBED_MAX_EMBD");
+    if (!grad_table || misaligned(grad_table, ts))
+        return fail(ZS_ERR_INVALID_ARGUMENT, "grad_table is null or not aligned to its type");
+    if (table_ld < n_embd || table_ld > (int64_t)1 << 30)
+        return fail(ZS_ERR_INVALID_ARGUMENT, "table_ld < n_embd or too large");
+    if (n_tokens > 0) {
+        if (!grad_out || !ids) return fail(ZS_ERR_INVALID_ARGUMENT, "grad_out or ids is null");
+        if (misaligned(grad_out, gs) || misaligned(ids, 4))
+            return fail(ZS_ERR_INVALID_ARGUMENT, "grad_out or ids not aligned to its type");
+        if (grad_ld < n_embd || grad_ld > (int64_t)1 << 30)
+            return fail(ZS_ERR_INVALID_ARGUMENT, "grad_ld < n_embd or too large");
+        if (!workspace || misaligned(workspace, 256) ||
+            workspace_bytes < embed_ws(n_tokens, n_embd).total)
+            return fail(ZS_ERR_INVALID_ARGUMENT,
+                        "workspace is null, not 256-byte aligned or smaller than "
+                        "zs_embed_backward_workspace says");
+    }
+    if (n_tokens == 0 && accumulate) return ZS_OK;
+    DeviceGuard g(h->device);
+    if (!g.ok) return fail(ZS_ERR_CUDA, "cudaSetDevice failed");
+    cudaStream_t st = (cudaStream_t)stream;
+    const EmbedWs w = embed_ws(n_tokens, n_embd);
+    uint8_t* ws = reinterpret_cast<uint8_t*>(workspace);
+    zs::EsArgs e;
+    std::memset(&e, 0, sizeof(e));
+    e.ids = ids;
+    e.n = (int32_t)n_tokens;
+    e.V = n_vocab;
+    // keys 0 .. n_vocab (the last for ids outside the table)
+    int bits = 1;
+    while (bits < 31 && ((int64_t)1 << bits) <= n_vocab) ++bits;
+    e.passes = (bits + 8) / 9;
+    e.digit_bits = (bits + e.passes - 1) / e.passes;
+    for (int i = 0; i < 2; ++i) {
+        e.key[i] = reinterpret_cast<uint32_t*>(ws + (2 * i) * w.pair_bytes);
+        e.pos[i] = reinterpret_cast<uint32_t*>(ws + (2 * i + 1) * w.pair_bytes);
+    }
+    if (!accumulate) {
+        e.z = reinterpret_cast<uint8_t*>(grad_table);
+        e.zsize = ts;
+        e.zld = table_ld;
+        e.zrows = table_ld == n_embd ? 1 : n_vocab;
+        e.zcols = table_ld == n_embd ? (int64_t)n_vocab * n_embd : n_embd;
+    }
+    {
+        // one cluster sorts; the others, one CTA per remaining SM, zero the table
+        LaunchScope scope(h, -1, st);
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = zs::kEsCl;
+        attr[0].val.clusterDim.y = 1;
+        attr[0].val.clusterDim.z = 1;
+        cudaLaunchConfig_t cfg;
+        std::memset(&cfg, 0, sizeof(cfg));
+        const int clusters = accumulate ? 1 : std::max(2, h->num_sms / zs::kEsCl);
+        cfg.gridDim = dim3((unsigned)(clusters * zs::kEsCl));
+        cfg.blockDim = dim3(zs::kEsThreads);
+        cfg.dynamicSmemBytes = sizeof(zs::EsSmem);
+        cfg.stream = st;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        ZS_CUDA(cudaLaunchKernelEx(&cfg, zs::zs_embed_sort_kernel, e));
+    }
+    if (n_tokens == 0) return ZS_OK;
+    zs::EbArgs b;
+    std::memset(&b, 0, sizeof(b));
+    b.grad = grad_out;
+    b.grad_ld = grad_ld;
+    b.n = (int32_t)n_tokens;
+    b.V = n_vocab;
+    b.E = n_embd;
+    b.key = e.key[e.passes & 1];
+    b.pos = e.pos[e.passes & 1];
+    b.scale = scale;
+    b.table = grad_table;
+    b.table_ld = table_ld;
+    b.accumulate = accumulate != 0;
+    b.part = reinterpret_cast<float*>(ws + w.part_at);
+    b.chunks = w.chunks;
+    if (grad_dtype == ZS_DTYPE_F32) return launch_embed_sum_in<float>(h, b, table_dtype, st);
+    if (grad_dtype == ZS_DTYPE_F16) return launch_embed_sum_in<__half>(h, b, table_dtype, st);
+    return launch_embed_sum_in<__nv_bfloat16>(h, b, table_dtype, st);
 }
 
 zs_status zs_shard_partial_bytes(int32_t batch, int32_t n_vocab_total, int32_t n_ranks,
