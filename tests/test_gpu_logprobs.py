@@ -385,11 +385,11 @@ def test_refusals(sampler):
     for y in (x.double(), x.cpu(), x.t(), x[0].expand(3, 100)):
         with pytest.raises(ValueError):
             sampler.logprobs(y)
-    for bad in (dict(top=-1), dict(temp=math.nan)):
-        with pytest.raises(SamplerError):
-            sampler.logprobs(x, ids, **bad)
     with pytest.raises(SamplerError):
-        sampler.logprobs(rand(1, 500, torch.float32), top=129)
+        sampler.logprobs(x, ids, temp=math.nan)
+    for y, top in ((x, -1), (rand(1, 500, torch.float32), 129)):
+        with pytest.raises(ValueError):
+            sampler.logprobs(y, top=top)
     with pytest.raises(SamplerError):
         sampler.logprobs(x, torch.zeros(4, 257, dtype=torch.int32, device="cuda"))
     g = torch.ones(4, device="cuda")

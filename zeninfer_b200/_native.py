@@ -27,6 +27,7 @@ EXPORTS = (
 )
 
 ZS_OK = 0
+LOGPROBS_MAX_TOP = 128  # ZS_LOGPROBS_MAX_TOP
 
 
 class ZsParams(C.Structure):

@@ -1187,7 +1187,7 @@ __global__ void __launch_bounds__(32 * kLmLogprobWarps) zs_lm_logprob_kernel(con
         st = lp_merge(st, {q.x, q.y, q.z}, c);
     }
     st = lp_warp_merge(st, c);
-    const double log_s = st.s == 0.0f ? -INFINITY : log((double)st.s);
+    const float log_s = lp_log_sum(st);
     const uint4* xr = reinterpret_cast<const uint4*>(a.xn + row * a.E);
     for (int j = 0; j < a.n_ids; ++j) {
         const int32_t id = a.ids[row * a.ids_ld + j];
@@ -1211,8 +1211,7 @@ __global__ void __launch_bounds__(32 * kLmLogprobWarps) zs_lm_logprob_kernel(con
     }
     if (lane == 0) {
         if (a.out_entropy) a.out_entropy[row] = lp_entropy(st, log_s);
-        if (a.out_lse)
-            a.out_lse[row] = st.s == 0.0f ? -INFINITY : (float)((double)st.m * (double)it + log_s);
+        if (a.out_lse) a.out_lse[row] = lp_lse(st, log_s, it);
     }
 }
 

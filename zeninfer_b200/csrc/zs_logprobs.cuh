@@ -30,8 +30,12 @@ namespace zs {
 
 constexpr int kLpMaxTop = 128;   // ZS_LOGPROBS_MAX_TOP
 constexpr int kLpMaxIds = 256;   // ZS_LOGPROBS_MAX_IDS
-constexpr int kLpMaxCl = 16;     // CTAs per row at most (one cluster)
+constexpr int kLpMaxCl = 8;      // CTAs per row at most (one portable cluster)
 constexpr int kLpCandCap = 1536; // candidates ranked at once
+constexpr int kLpUnroll = 4;     // vectors in flight per thread
+constexpr int kLpSegVecs = 32 * kLpUnroll;  // a segment: what a warp takes at a time, 2 KB
+constexpr int kLpMaxSegs = 1024; // segment maxima a CTA keeps (2 MB of logits)
+constexpr int kLpMaxHits = 512;
 constexpr float kLpFloor = -200.0f;
 constexpr float kLpLog2e = 1.4426950408889634f;
 constexpr double kLpLn2 = 0.6931471805599453;
@@ -130,6 +134,98 @@ __device__ __forceinline__ LpCut lp_cut(const T* p, int n) {
     return c;
 }
 
+// ---- pairs of f32 (one instruction for two) ----
+__device__ __forceinline__ uint64_t f2_make(float lo, float hi) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ void f2_split(uint64_t v, float& lo, float& hi) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+__device__ __forceinline__ uint64_t f2_add(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t f2_mul(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+
+// ---- pairs of 16-bit values ----
+template <typename T>
+struct LpPair;
+template <>
+struct LpPair<__half> {
+    static __device__ __forceinline__ uint32_t max(uint32_t a, uint32_t b) {
+        uint32_t r;
+        asm("max.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+        return r;
+    }
+    static __device__ __forceinline__ uint32_t max_nan(uint32_t a, uint32_t b) {
+        uint32_t r;
+        asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+        return r;
+    }
+    static __device__ __forceinline__ uint32_t down(float v) {  // v rounded down, twice
+        const uint32_t h = __half_as_ushort(__float2half_rd(v));
+        return h | (h << 16);
+    }
+    static __device__ __forceinline__ void split(uint32_t w, float& lo, float& hi) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+        lo = f.x;
+        hi = f.y;
+    }
+};
+template <>
+struct LpPair<__nv_bfloat16> {
+    static __device__ __forceinline__ uint32_t max(uint32_t a, uint32_t b) {
+        uint32_t r;
+        asm("max.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+        return r;
+    }
+    static __device__ __forceinline__ uint32_t max_nan(uint32_t a, uint32_t b) {
+        uint32_t r;
+        asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+        return r;
+    }
+    static __device__ __forceinline__ uint32_t down(float v) {
+        const uint32_t h = __bfloat16_as_ushort(__float2bfloat16_rd(v));
+        return h | (h << 16);
+    }
+    static __device__ __forceinline__ void split(uint32_t w, float& lo, float& hi) {
+        lo = __uint_as_float(w << 16);
+        hi = __uint_as_float(w & 0xffff0000u);
+    }
+};
+
+// The largest value of a 16-byte vector (NaN ignored).
+__device__ __forceinline__ float lp_vec_max(const uint4& q, float) {
+    return fmaxf(fmaxf(__uint_as_float(q.x), __uint_as_float(q.y)),
+                 fmaxf(__uint_as_float(q.z), __uint_as_float(q.w)));
+}
+template <typename T>
+__device__ __forceinline__ float lp_vec_max(const uint4& q, T) {
+    float lo, hi;
+    LpPair<T>::split(LpPair<T>::max(LpPair<T>::max(q.x, q.y), LpPair<T>::max(q.z, q.w)), lo, hi);
+    return fmaxf(lo, hi);
+}
+
+// The largest value of a warp: an integer reduction of a monotone map of the values
+// (the f32 one measured 230 cycles).  NaN, which no maximum here is, would not be ignored.
+__device__ __forceinline__ float lp_warp_max(float v) {
+    const int i = __float_as_int(v);
+    const int m = __reduce_max_sync(kFull, i < 0 ? i ^ 0x7fffffff : i);
+    return __int_as_float(m < 0 ? m ^ 0x7fffffff : m);
+}
+
 // ---- running statistics ----
 struct LpStat {
     float m, s, w;  // max, sum of 2^t, sum of 2^t t with t = (x - m) c
@@ -153,13 +249,12 @@ __device__ __forceinline__ LpStat lp_merge(LpStat a, LpStat b, float c) {
     return a;
 }
 __device__ __forceinline__ LpStat lp_warp_merge(LpStat a, float c) {
+    const float m = lp_warp_max(a.m);
+    if (m > a.m) lp_raise(a, m, c);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
-        LpStat b;
-        b.m = __shfl_xor_sync(kFull, a.m, o);
-        b.s = __shfl_xor_sync(kFull, a.s, o);
-        b.w = __shfl_xor_sync(kFull, a.w, o);
-        a = lp_merge(a, b, c);
+        a.s += __shfl_xor_sync(kFull, a.s, o);
+        a.w += __shfl_xor_sync(kFull, a.w, o);
     }
     return a;
 }
@@ -174,20 +269,116 @@ __device__ __forceinline__ void lp_scalar(LpStat& a, float v, float c) {
     lp_add(a, v, a.m == -INFINITY ? 0.0f : a.m, c);
 }
 
+// A statistic over pairs: two sums side by side.
+struct LpStat2 {
+    float m;
+    uint64_t s, w;
+};
+__device__ __forceinline__ void lp_raise2(LpStat2& a, float m, float c) {
+    const float t = fmaxf((a.m - m) * c, kLpFloor);
+    const float f = fast_exp2(t);
+    const uint64_t f2 = f2_make(f, f), t2 = f2_make(t, t);
+    a.w = f2_mul(f2, f2_fma(a.s, t2, a.w));
+    a.s = f2_mul(a.s, f2);
+    a.m = m;
+}
+__device__ __forceinline__ LpStat lp_single(const LpStat2& a) {
+    LpStat r;
+    float lo, hi;
+    r.m = a.m;
+    f2_split(a.s, lo, hi);
+    r.s = lo + hi;
+    f2_split(a.w, lo, hi);
+    r.w = lo + hi;
+    return r;
+}
+template <bool CLAMP>
+__device__ __forceinline__ void lp_add2(LpStat2& a, float lo, float hi, uint64_t minus_base,
+                                        uint64_t c2) {
+    uint64_t t2 = f2_mul(f2_add(f2_make(lo, hi), minus_base), c2);
+    float t0, t1;
+    f2_split(t2, t0, t1);
+    if (CLAMP) {
+        t0 = lp_max_nan(t0, kLpFloor);
+        t1 = lp_max_nan(t1, kLpFloor);
+        t2 = f2_make(t0, t1);
+    }
+    const uint64_t e2 = f2_make(fast_exp2(t0), fast_exp2(t1));
+    a.s = f2_add(a.s, e2);
+    a.w = f2_fma(e2, t2, a.w);
+}
+
+// U vectors into a statistic whose maximum is at least theirs.
+template <int U>
+__device__ __forceinline__ void lp_add_vecs(LpStat2& a, const uint4 (&q)[U], float c, uint32_t,
+                                            float) {
+    const float base = a.m == -INFINITY ? 0.0f : a.m;
+    const uint64_t mb = f2_make(-base, -base), c2 = f2_make(c, c);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        lp_add2<true>(a, __uint_as_float(q[u].x), __uint_as_float(q[u].y), mb, c2);
+        lp_add2<true>(a, __uint_as_float(q[u].z), __uint_as_float(q[u].w), mb, c2);
+    }
+}
+// 16-bit values are clamped in pairs before they are widened, at `low`, the maximum less
+// 180 / c rounded down to the type: 2^t is 0 there.  Where that is not finite (low
+// 0xff80ff80 or 0xfc00fc00: next to the type's lowest value) t is clamped instead.
+template <int U, typename T>
+__device__ __forceinline__ void lp_add_vecs(LpStat2& a, const uint4 (&q)[U], float c, uint32_t low,
+                                            T) {
+    const float base = a.m == -INFINITY ? 0.0f : a.m;
+    const uint64_t mb = f2_make(-base, -base), c2 = f2_make(c, c);
+    if (low != lp_fill(T()).x) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const uint32_t w[4] = {q[u].x, q[u].y, q[u].z, q[u].w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                float lo, hi;
+                LpPair<T>::split(LpPair<T>::max_nan(w[i], low), lo, hi);
+                lp_add2<false>(a, lo, hi, mb, c2);
+            }
+        }
+    } else {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const uint32_t w[4] = {q[u].x, q[u].y, q[u].z, q[u].w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                float lo, hi;
+                LpPair<T>::split(w[i], lo, hi);
+                lp_add2<true>(a, lo, hi, mb, c2);
+            }
+        }
+    }
+}
+__device__ __forceinline__ uint32_t lp_low(float, float, float) { return 0u; }
+template <typename T>
+__device__ __forceinline__ uint32_t lp_low(float m, float c, T) {
+    return LpPair<T>::down(__fsub_rd(m, 180.0f / c));  // always below m
+}
+
 // 1 / temp as the sampler takes it (1 for greedy rows).
 __device__ __forceinline__ float lp_inv_temp(float temp, const float* row_temp, int64_t row) {
     const float t = row_temp ? row_temp[row] : temp;
     return t <= 0.0f ? 1.0f : 1.0f / t;
 }
 
-// log p of a value from the row's statistics, in f64 (one value per row and id).
-__device__ __forceinline__ float lp_value(float x, float m, double log_s, float it) {
-    if (log_s == -INFINITY) return -INFINITY;
-    return (float)(((double)x - (double)m) * (double)it - log_s);
+// log p of a value from the row's statistics.  Both terms are at most 0, so the f32
+// logarithm's relative error is the result's.
+__device__ __forceinline__ float lp_log_sum(const LpStat& a) {
+    return a.s == 0.0f ? -INFINITY : logf(a.s);
 }
-__device__ __forceinline__ float lp_entropy(const LpStat& a, double log_s) {
+__device__ __forceinline__ float lp_value(float x, float m, float log_s, float it) {
+    if (log_s == -INFINITY) return -INFINITY;
+    return (float)(((double)x - (double)m) * (double)it - (double)log_s);
+}
+__device__ __forceinline__ float lp_lse(const LpStat& a, float log_s, float it) {
+    return a.s == 0.0f ? -INFINITY : (float)((double)a.m * (double)it + (double)log_s);
+}
+__device__ __forceinline__ float lp_entropy(const LpStat& a, float log_s) {
     if (a.s == 0.0f) return 0.0f;
-    const float h = (float)(log_s - kLpLn2 * (double)a.w / (double)a.s);
+    const float h = log_s - 0.6931471805599453f * (a.w / a.s);  // two terms of one sign
     return h < 0.0f ? 0.0f : h;
 }
 
@@ -211,123 +402,185 @@ struct LpArgs {
     int32_t cl;          // CTAs per row
 };
 
-// Number of keys of a descending list that are greater than `key`.
-__device__ __forceinline__ int lp_above(const uint64_t* list, int n, uint64_t key) {
-    int lo = 0, hi = n;
-    while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        if (list[mid] > key)
-            lo = mid + 1;
-        else
-            hi = mid;
+// 32 keys of a warp that form a bitonic sequence, into descending order.
+__device__ __forceinline__ uint32_t lp_bitonic(uint32_t key, int lane) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        const uint32_t other = __shfl_xor_sync(kFull, key, o);
+        key = (lane & o) == 0 ? max(key, other) : min(key, other);
     }
-    return lo;
+    return key;
 }
-
-// The 32 keys of a warp in descending order (bitonic).
-__device__ __forceinline__ void lp_warp_sort(uint64_t& key, uint32_t& tag, int lane) {
+// The 32 keys of a warp in descending order.
+__device__ __forceinline__ uint32_t lp_warp_sort(uint32_t key, int lane) {
 #pragma unroll
     for (int size = 2; size <= 32; size <<= 1) {
 #pragma unroll
         for (int o = size >> 1; o > 0; o >>= 1) {
-            const uint64_t ok = __shfl_xor_sync(kFull, key, o);
-            const uint32_t ot = __shfl_xor_sync(kFull, tag, o);
-            const bool lower = (lane & o) == 0;
-            const bool desc = (lane & size) == 0 || size == 32;
-            const bool take = (lower == desc) ? ok > key : ok < key;
-            if (take) {
-                key = ok;
-                tag = ot;
-            }
+            const uint32_t other = __shfl_xor_sync(kFull, key, o);
+            const bool greater = ((lane & o) == 0) == ((lane & size) == 0 || size == 32);
+            key = greater ? max(key, other) : min(key, other);
         }
     }
+    return key;
 }
+
+// A thread's rough key: the upper 20 bits of its maximum's order, then 4095 less its
+// number in the cluster (at most kLpMaxCl x 512 threads), so that keys differ.
+constexpr int kLpCodeBits = 12;
+constexpr uint32_t kLpCodeMask = (1u << kLpCodeBits) - 1u;
 
 template <int NT>
 struct LpTopSmem {
-    uint64_t warp_keys[NT];               // each warp's sorted thread keys
-    uint32_t warp_tags[NT];
-    uint64_t cta_keys[kLpMaxTop];         // this CTA's best, read by the leader
-    uint32_t cta_tags[kLpMaxTop];
-    uint64_t all_keys[kLpMaxCl * kLpMaxTop];
-    uint32_t all_tags[kLpMaxCl * kLpMaxTop];
-    uint64_t sel_keys[kLpMaxTop];
-    uint32_t sel_tags[kLpMaxTop];         // source CTA << 16 | thread
+    static_assert(kLpMaxCl * NT <= 1 << kLpCodeBits, "thread numbers fit the rough keys");
+    uint32_t tree[NT / 32][32];    // one level of the merge
+    uint32_t lists[NT / 32][32];   // each warp's sorted thread keys
+    uint32_t cta_keys[kLpMaxTop];  // this CTA's best, read by the leader
+    uint32_t sel_keys[kLpMaxTop];  // the row's best threads
+    uint64_t exact[NT];            // every thread's key (value, first id of its vector)
     uint64_t cand[kLpCandCap];
+    float seg_max[kLpMaxSegs];     // of each segment of this CTA's slice
+    int32_t hits[kLpMaxHits];      // segments to read again: their first vector in the row
     uint64_t red[NT / 32];
-    int ncta, nsel, ncand;
+    int ncand, nhits;
 };
 
+// The k best keys (rounded up to a multiple of 32, 0 where there are none) of nl
+// descending lists, a power of two and at most one per warp, into `out`: at(i) is key i
+// of this warp's list (0 past its end).  32 keys per round: a tree of merges takes the
+// best 32 of the lists' next 32, and each list moves on past those taken from it.
+template <int NT, class At>
+__device__ __forceinline__ void lp_merge_lists(LpTopSmem<NT>& tp, int nl, int k, uint32_t* out,
+                                               int warp, int lane, At at) {
+    int taken = 0;
+    for (int r0 = 0; r0 < k; r0 += 32) {
+        const uint32_t mine = warp < nl ? at(taken + lane) : 0u;
+        uint32_t key = mine;
+        for (int n = nl >> 1; n >= 1; n >>= 1) {
+            if (warp >= n && warp < 2 * n) tp.tree[warp][lane] = key;
+            __syncthreads();
+            // descending against ascending: the larger of each pair are the best 32 of
+            // both, a bitonic sequence
+            if (warp < n) key = lp_bitonic(max(key, tp.tree[warp + n][31 - lane]), lane);
+        }
+        if (warp == 0) out[r0 + lane] = key;
+        __syncthreads();
+        if (r0 + 32 < k)
+            taken += __popc(__ballot_sync(kFull, mine != 0u && mine >= out[r0 + 31]));
+    }
+}
+
+// The two halves of a cluster barrier (every thread of every CTA of the cluster).
+__device__ __forceinline__ void cluster_arrive() {
+    asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_wait() {
+    asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+}
+
+// A vector of the row: kept in L2 when some segments are read again, else read once.
+template <bool AGAIN>
+__device__ __forceinline__ uint4 lp_stream(const uint4* p) {
+    return AGAIN ? __ldcg(p) : __ldcs(p);
+}
+
 // One row per cluster of a.cl CTAs (one CTA when a.cl is 1).  The row is streamed
-// once with 16-byte loads, kUnroll in flight per thread; the CTAs' statistics meet in
-// the leader (rank 0) through distributed shared memory in rank order, so no scratch,
-// no atomics and a fixed summation order.
+// once with 16-byte loads: a warp takes a segment of kLpUnroll x 32 vectors (2 KB) at a
+// time and loads its next one before it works on this.  The CTAs'
+// statistics meet in the leader (rank 0) through distributed shared memory in rank
+// order, so no scratch, no global atomics and a fixed summation order.
 //
-// Alternatives (TOP).  Each thread's elements form a group whose best key (value
-// desc, id asc) the running maximum already gives, up to the vector it was first seen
-// in.  The k best elements all lie in the k groups with the best such keys: if an
-// element's group is not among them, k groups rank before it and each holds an element
-// that does.  So the pass keeps one position per thread, the k best groups are found
-// at the end (warp sort, then ranks by binary search), and only those k groups (a
-// few hundred elements) are read again, from L2.  Should the candidates not suffice
-// (NaN groups) or not fit, the leader takes the k best one after another from the row.
+// Alternatives (TOP).  Every thread keeps its maximum and the first vector it was seen
+// in, and the warp every segment's maximum.  The k-th best of the threads' maxima is a
+// lower bound of the row's k-th best value: k threads hold an element at or above it.
+// The leader finds it by merging the threads' sorted rough keys (32 bits: one shuffle
+// and one min or max per step; a bound may be a little low), and reads again (from L2)
+// only the segments whose maximum reaches it, about k of them; what reaches it there is
+// ranked by counting.  Where too many do (ties), the bound is taken exactly, with the
+// id: the least of the k threads' exact keys (value desc, id asc).  Should there still
+// be too many, or too few (NaN among the threads' vectors), the leader takes the k best
+// one after another from the row.
 template <typename T, int NT, bool TOP>
 __global__ void __launch_bounds__(NT, 1024 / NT) zs_logprobs_kernel(const LpArgs a) {
     namespace cg = cooperative_groups;
     constexpr int N = LpVec<T>::N;
-    constexpr int kUnroll = 4;
-    extern __shared__ __align__(16) uint8_t lp_raw[];
+    constexpr int kUnroll = kLpUnroll;
     __shared__ LpStat warp_stat[NT / 32];
     __shared__ LpStat cta_stat;
     cg::cluster_group cluster = cg::this_cluster();
-    const int rank = a.cl > 1 ? (int)cluster.block_rank() : 0;
-    const int64_t row = blockIdx.x / a.cl;
+    const int cl = a.cl;
+    const int rank = cl > 1 ? (int)cluster.block_rank() : 0;
+    const int64_t row = blockIdx.x / cl;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const T* x = reinterpret_cast<const T*>(a.logits) + row * a.ld;
+
+    // the leader's given id and its logit, in flight during the pass
+    float given = 0.0f;
+    bool given_in = false;
+    if (rank == 0 && tid < a.n_ids) {
+        const int32_t id = a.ids[row * a.ids_ld + tid];
+        given_in = id >= 0 && id < a.n;
+        if (given_in) given = lp_float(x[id]);
+    }
     const float it = lp_inv_temp(a.temp, a.row_temp, row);
     const float c = it * kLpLog2e;
 
     const LpCut cut = lp_cut(x, a.n);
     const uint4* xv = reinterpret_cast<const uint4*>(x + cut.head);
-    const int v0 = (int)((int64_t)cut.nvec * rank / a.cl);
-    const int v1 = (int)((int64_t)cut.nvec * (rank + 1) / a.cl);
+    const int v0 = (int)((int64_t)cut.nvec * rank / cl);
+    const int v1 = (int)((int64_t)cut.nvec * (rank + 1) / cl);
 
-    LpStat st = lp_empty();
+    LpStat2 st2 = {-INFINITY, 0ull, 0ull};
+    uint32_t low = lp_fill(T()).x;
     int pos = -1;  // first id of the vector that holds this thread's maximum
+    float edge = -INFINITY;
+    bool has_edge = false;
     if (rank == 0 && tid < cut.head) {
-        lp_scalar(st, lp_float(x[tid]), c);
+        edge = lp_float(x[tid]);
+        has_edge = true;
         pos = tid;
+        if (TOP && edge > st2.m) lp_raise2(st2, edge, c);
     }
-    if (TOP && pos < 0 && v0 + tid < v1) pos = cut.head + (v0 + tid) * N;
-    for (int i = v0 + tid; i < v1; i += NT * kUnroll) {
-        uint4 q[kUnroll];
+    __shared__ LpTopSmem<TOP ? NT : 32> tp;
+    const int first = v0 + warp * 32 * kUnroll + lane;
+    if (TOP && pos < 0 && first < v1) pos = cut.head + first * N;
+    const bool keep_segs = TOP && (v1 - v0 + kLpSegVecs - 1) / kLpSegVecs <= kLpMaxSegs;
+    uint4 q[kUnroll];
 #pragma unroll
-        for (int u = 0; u < kUnroll; ++u)
-            q[u] = i + u * NT < v1 ? __ldcs(xv + i + u * NT) : lp_fill(T());
-        float m = st.m;
+    for (int u = 0; u < kUnroll; ++u)
+        q[u] = first + u * 32 < v1 ? lp_stream<TOP>(xv + first + u * 32) : lp_fill(T());
+    for (int i = first; i - lane < v1; i += NT * kUnroll) {
+        uint4 next[kUnroll];
 #pragma unroll
         for (int u = 0; u < kUnroll; ++u) {
-            float v[N];
-            lp_unpack(q[u], v, T());
-            float b = v[0];
+            const int j = i + NT * kUnroll + u * 32;
+            next[u] = j < v1 ? lp_stream<TOP>(xv + j) : lp_fill(T());
+        }
+        float m = st2.m, seg = -INFINITY;
 #pragma unroll
-            for (int j = 1; j < N; ++j) b = fmaxf(b, v[j]);
+        for (int u = 0; u < kUnroll; ++u) {
+            const float b = lp_vec_max(q[u], T());
             if (b > m) {
                 m = b;
-                if (TOP) pos = cut.head + (i + u * NT) * N;
+                if (TOP) pos = cut.head + (i + u * 32) * N;
             }
+            if (TOP) seg = fmaxf(seg, b);
         }
-        if (m > st.m) lp_raise(st, m, c);
-        const float base = st.m == -INFINITY ? 0.0f : st.m;
-#pragma unroll
-        for (int u = 0; u < kUnroll; ++u) {
-            float v[N];
-            lp_unpack(q[u], v, T());
-#pragma unroll
-            for (int j = 0; j < N; ++j) lp_add(st, v[j], base, c);
+        if (TOP && keep_segs) {
+            seg = lp_warp_max(seg);
+            if (lane == 0) tp.seg_max[(i - v0) / kLpSegVecs] = seg;
         }
+        if (m > st2.m) {
+            lp_raise2(st2, m, c);
+            low = lp_low(m, c, T());
+        }
+        lp_add_vecs(st2, q, c, low, T());
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) q[u] = next[u];
     }
-    if (rank == a.cl - 1 && tid < cut.tail) {
+    LpStat st = lp_single(st2);
+    if (has_edge) lp_scalar(st, edge, c);
+    if (rank == cl - 1 && tid < cut.tail) {
         const int id = cut.head + cut.nvec * N + tid;
         const float v = lp_float(x[id]);
         if (TOP && (pos < 0 || v > st.m)) pos = id;
@@ -336,93 +589,90 @@ __global__ void __launch_bounds__(NT, 1024 / NT) zs_logprobs_kernel(const LpArgs
     const float best = st.m;  // this thread's own maximum
 
     // ---- statistics: warp, CTA, cluster ----
+    constexpr int kWarps = NT / 32;
+    const int k = a.k;
     st = lp_warp_merge(st, c);
     if (lane == 0) warp_stat[warp] = st;
-    __syncthreads();
-    if (warp == 0) {
-        LpStat t = lane < NT / 32 ? warp_stat[lane] : lp_empty();
-        t = lp_warp_merge(t, c);
-        if (lane == 0) cta_stat = t;
-    }
-
-    LpTopSmem<NT>& tp = *reinterpret_cast<LpTopSmem<NT>*>(lp_raw);
-    const int k = a.k;
-    if (TOP) {
-        // this CTA's k best groups
-        uint64_t key = pos >= 0 ? make_key(best, pos) : 0ull;
-        uint32_t tag = (uint32_t)tid;
-        lp_warp_sort(key, tag, lane);
-        tp.warp_keys[tid] = key;
-        tp.warp_tags[tid] = tag;
-        if (tid == 0) {
-            tp.ncta = 0;
-            tp.ncand = 0;
+    if constexpr (TOP) {
+        // this CTA's k best threads
+        uint32_t key = 0u;
+        uint64_t full = 0ull;
+        if (pos >= 0) {
+            full = make_key(best, pos);
+            key = ((uint32_t)(full >> 32) & ~kLpCodeMask) | (kLpCodeMask - (uint32_t)(rank * NT + tid));
         }
+        tp.exact[tid] = full;
+        key = lp_warp_sort(key, lane);
+        if (k > 32) tp.lists[warp][lane] = key;
+        if (tid == 0) tp.ncand = tp.nhits = 0;
+        lp_merge_lists<NT>(tp, kWarps, k, tp.cta_keys, warp, lane, [&](int i) {
+            return i == lane ? key : i < 32 ? tp.lists[warp][i] : 0u;
+        });
+    } else {
         __syncthreads();
-        if (key != 0ull) {
-            int r = lane;
-            for (int w = 0; w < NT / 32 && r < k; ++w)
-                if (w != warp) r += lp_above(tp.warp_keys + w * 32, 32, key);
-            if (r < k) {
-                tp.cta_keys[r] = key;
-                tp.cta_tags[r] = tag;
-                atomicAdd(&tp.ncta, 1);
-            }
+    }
+    if (cl == 1 || warp == 0) {  // one CTA: every warp for itself
+        st = lp_warp_merge(lane < kWarps ? warp_stat[lane] : lp_empty(), c);
+        if (cl > 1 && lane == 0) cta_stat = st;
+    }
+    if (cl > 1) {
+        cluster_arrive();
+        cluster_wait();
+        if (rank != 0) {
+            cluster_arrive();
+            cluster_wait();  // the leader has read this CTA's shared memory
+            return;
+        }
+        st = lane < cl ? *cluster.map_shared_rank(&cta_stat, lane) : lp_empty();
+    }
+    constexpr int kSegAhead = 4;  // segment maxima a lane has in flight
+    float ahead[kSegAhead];
+    if constexpr (TOP) {
+        if (cl > 1) {
+            // the row's k best threads; their CTAs' segment maxima arrive meanwhile
+            const LpTopSmem<NT>* from = cluster.map_shared_rank(&tp, warp < cl ? warp : 0);
+#pragma unroll
+            for (int u = 0; u < kSegAhead; ++u) ahead[u] = from->seg_max[lane + 32 * u];
+            const uint32_t* list = from->cta_keys;
+            lp_merge_lists<NT>(tp, cl, k, tp.sel_keys, warp, lane,
+                               [&](int i) { return i < k ? list[i] : 0u; });
         }
     }
-    if (a.cl > 1)
-        cluster.sync();
-    else
-        __syncthreads();
-    if (rank != 0) {
-        cluster.sync();  // the leader has read this CTA's shared memory
-        return;
-    }
-
-    st = cta_stat;
-    if (a.cl > 1) {
-        st = lane < a.cl ? *cluster.map_shared_rank(&cta_stat, lane) : lp_empty();
-        st = lp_warp_merge(st, c);
-    }
-    if (TOP) {
-        // the row's k best groups
-        const int cl = a.cl;
-        int total = 0;
-        for (int r = 0; r < cl; ++r) {
-            const LpTopSmem<NT>* o = cl > 1 ? cluster.map_shared_rank(&tp, r) : &tp;
-            const int nr = o->ncta;
-            total += nr;
-            for (int i = tid; i < k; i += NT) {
-                tp.all_keys[r * k + i] = i < nr ? o->cta_keys[i] : 0ull;
-                tp.all_tags[r * k + i] = i < nr ? ((uint32_t)r << 16) | o->cta_tags[i] : 0u;
+    if (cl > 1) st = lp_warp_merge(st, c);
+    const float log_s = lp_log_sum(st);
+    if constexpr (TOP) {
+        const uint32_t* sel = cl > 1 ? tp.sel_keys : tp.cta_keys;
+        const int vec_end = cut.head + cut.nvec * N;
+        // Candidates are the elements whose key is at least floor_key (0: all).
+        uint64_t floor_key = (uint64_t)(sel[k - 1] & ~kLpCodeMask) << 32;
+        // the segments that may hold one: warp w looks through slice w, or every warp
+        // through a part of the only slice
+        auto find = [&](bool loaded) {
+            const int r = cl > 1 ? warp : 0, parts = cl > 1 ? 1 : kWarps;
+            const int b0 = (int)((int64_t)cut.nvec * r / cl), b1 = (int)((int64_t)cut.nvec * (r + 1) / cl);
+            const int nseg = r < cl ? (b1 - b0 + kLpSegVecs - 1) / kLpSegVecs : 0;
+            const bool kept = nseg <= kLpMaxSegs;
+            const float* seg = (cl > 1 && r < cl ? cluster.map_shared_rank(&tp, r) : &tp)->seg_max;
+            for (int i0 = (cl > 1 ? 0 : warp * 32 * kSegAhead); i0 < nseg; i0 += parts * 32 * kSegAhead) {
+                if (!loaded || i0 > 0) {
+#pragma unroll
+                    for (int u = 0; u < kSegAhead; ++u) {
+                        const int i = i0 + lane + u * 32;
+                        ahead[u] = kept && i < nseg ? seg[i] : 0.0f;
+                    }
+                }
+#pragma unroll
+                for (int u = 0; u < kSegAhead; ++u) {
+                    const int i = i0 + lane + u * 32;
+                    const int v = b0 + i * kLpSegVecs;  // the segment's first vector
+                    if (i < nseg && (!kept || make_key(ahead[u], cut.head + v * N) >= floor_key)) {
+                        const int at = atomicAdd(&tp.nhits, 1);
+                        if (at < kLpMaxHits) tp.hits[at] = v;
+                    }
+                }
             }
-        }
-        const int nsel = min(k, total);
-        if (cl > 1)
-            cluster.sync();
-        else
             __syncthreads();
-        for (int i = tid; i < cl * k; i += NT) {
-            const uint64_t key = tp.all_keys[i];
-            if (key == 0ull) continue;
-            int r = i % k;
-            for (int o = 0; o < cl && r < nsel; ++o)
-                if (o != i / k) r += lp_above(tp.all_keys + o * k, k, key);
-            if (r < nsel) {
-                tp.sel_keys[r] = key;
-                tp.sel_tags[r] = tp.all_tags[i];
-            }
-        }
-        __syncthreads();
-        // Every element at or above the last group's best is a candidate; its key is
-        // known up to the id within its vector.
-        uint64_t floor_key = 0ull;
-        if (nsel == k) {
-            const uint64_t last = tp.sel_keys[k - 1];
-            const int id = key_id(last);
-            const int span = (id >= cut.head && id < cut.head + cut.nvec * N) ? N : 1;
-            floor_key = (last & 0xffffffff00000000ull) | (uint64_t)(~(uint32_t)(id + span - 1));
-        }
+        };
         auto offer = [&](float v, int id) {
             const uint64_t key = make_key(v, id);
             if (key >= floor_key) {
@@ -430,37 +680,82 @@ __global__ void __launch_bounds__(NT, 1024 / NT) zs_logprobs_kernel(const LpArgs
                 if (at < kLpCandCap) tp.cand[at] = key;
             }
         };
-        for (int g = warp; g < nsel; g += NT / 32) {
-            const int src = (int)(tp.sel_tags[g] >> 16), t = (int)(tp.sel_tags[g] & 0xffffu);
-            const int b0 = (int)((int64_t)cut.nvec * src / cl);
-            const int b1 = (int)((int64_t)cut.nvec * (src + 1) / cl);
-            for (int i = b0 + t + lane * NT; i < b1; i += 32 * NT) {
-                const uint4 q = xv[i];
-                float v[N];
-                lp_unpack(q, v, T());
+        auto collect = [&] {
+            const int nhits = tp.nhits;
+            const float low_value = key_value(floor_key);  // NaN when every element is offered
+            const volatile int* full = &tp.ncand;
+            for (int h = warp; h < nhits && nhits <= kLpMaxHits && *full <= kLpCandCap; h += kWarps) {
+                const int seg0 = tp.hits[h];
+                int end = cut.nvec;  // of the slice the segment belongs to
+                for (int r = cl - 1; r > 0 && (int)((int64_t)cut.nvec * r / cl) > seg0; --r)
+                    end = (int)((int64_t)cut.nvec * r / cl);
+                uint4 hq[kUnroll];
 #pragma unroll
-                for (int j = 0; j < N; ++j) offer(v[j], cut.head + i * N + j);
+                for (int u = 0; u < kUnroll; ++u)
+                    if (seg0 + lane + u * 32 < end) hq[u] = xv[seg0 + lane + u * 32];
+#pragma unroll 1
+                for (int v = seg0 + lane; v < min(end, seg0 + kLpSegVecs); v += 32) {
+                    // a loop, not kUnroll copies of code that runs once
+                    if (lp_vec_max(hq[0], T()) >= low_value || low_value != low_value) {
+                        float e[N];
+                        lp_unpack(hq[0], e, T());
+#pragma unroll
+                        for (int j = 0; j < N; ++j) offer(e[j], cut.head + v * N + j);
+                    }
+#pragma unroll
+                    for (int u = 0; u + 1 < kUnroll; ++u) hq[u] = hq[u + 1];
+                }
             }
-            if (lane == 0 && src == 0 && t < cut.head) offer(lp_float(x[t]), t);
-            if (lane == 0 && src == cl - 1 && t < cut.tail) {
-                const int id = cut.head + cut.nvec * N + t;
-                offer(lp_float(x[id]), id);
-            }
-        }
-        __syncthreads();
-        const int nc = tp.ncand;
-        const double log_s = log((double)st.s) + 0.0;
-        const double ls = st.s == 0.0f ? -INFINITY : log_s;
-        auto put = [&](int r, uint64_t key) {
-            const int id = key_id(key);
-            a.top_ids[row * a.top_ld + r] = id;
-            a.top_logp[row * a.top_ld + r] = lp_value(lp_float(x[id]), st.m, ls, it);
+            if (tid < cut.head) offer(lp_float(x[tid]), tid);
+            if (tid < cut.tail) offer(lp_float(x[vec_end + tid]), vec_end + tid);
+            __syncthreads();
         };
-        if (nc >= k && nc <= kLpCandCap) {
+        // Among masked tokens everything ties, so there the exact bound is taken at once.
+        bool rough = (uint32_t)(floor_key >> 32) > 0x007fffffu;  // the order of -inf
+        if (rough) {
+            find(cl > 1);
+            collect();
+            rough = tp.nhits <= kLpMaxHits && tp.ncand <= kLpCandCap;
+        }
+        if (!rough) {
+            // the exact bound, up to the id within its vector
+            uint64_t low = ~0ull;
+            for (int i = tid; i < k; i += NT) {
+                uint64_t key = 0ull;
+                if (sel[i] != 0u) {
+                    const int code = (int)(kLpCodeMask - (sel[i] & kLpCodeMask));
+                    key = (cl > 1 ? cluster.map_shared_rank(&tp, code / NT) : &tp)->exact[code % NT];
+                    const int id = key_id(key);
+                    const int span = (id >= cut.head && id < vec_end) ? N : 1;
+                    key = (key & 0xffffffff00000000ull) | (uint64_t)(~(uint32_t)(id + span - 1));
+                }
+                low = key < low ? key : low;
+            }
+            __syncthreads();
+            if (tid == 0) {
+                tp.red[0] = ~0ull;
+                tp.ncand = tp.nhits = 0;
+            }
+            __syncthreads();
+            if (tid < k) atomicMin(reinterpret_cast<unsigned long long*>(&tp.red[0]), low);
+            __syncthreads();
+            floor_key = tp.red[0];
+            find(false);
+            collect();
+        }
+        if (cl > 1) cluster_arrive();  // the other CTAs may go
+        const int nhits = tp.nhits;
+        const int nc = tp.ncand;
+        auto put = [&](int r, uint64_t key) {
+            a.top_ids[row * a.top_ld + r] = key_id(key);
+            a.top_logp[row * a.top_ld + r] = lp_value(key_value(key), st.m, log_s, it);
+        };
+        if (nc >= k && nc <= kLpCandCap && nhits <= kLpMaxHits) {
             for (int i = tid; i < nc; i += NT) {
                 const uint64_t key = tp.cand[i];
                 int r = 0;
-                for (int j = 0; j < nc && r < k; ++j) r += tp.cand[j] > key ? 1 : 0;
+#pragma unroll 8
+                for (int j = 0; j < nc; ++j) r += tp.cand[j] > key ? 1 : 0;
                 if (r < k) put(r, key);
             }
         } else {
@@ -485,25 +780,21 @@ __global__ void __launch_bounds__(NT, 1024 / NT) zs_logprobs_kernel(const LpArgs
                 prev = b;
             }
         }
-    } else if (a.cl > 1) {
-        cluster.sync();
+    } else {
+        if (cl > 1) cluster_arrive();
     }
 
     // ---- the row's numbers ----
-    const double log_s = st.s == 0.0f ? -INFINITY : log((double)st.s);
-    for (int j = tid; j < a.n_ids; j += NT) {
-        const int32_t id = a.ids[row * a.ids_ld + j];
-        a.out_logp[row * a.n_ids + j] =
-            (id < 0 || id >= a.n) ? 0.0f : lp_value(lp_float(x[id]), st.m, log_s, it);
-    }
+    if (tid < a.n_ids) a.out_logp[row * a.n_ids + tid] = given_in ? lp_value(given, st.m, log_s, it) : 0.0f;
     if (tid == 0) {
         const float h = lp_entropy(st, log_s);
         if (a.out_entropy) a.out_entropy[row] = h;
-        if (a.out_lse)
-            a.out_lse[row] = st.s == 0.0f ? -INFINITY : (float)((double)st.m * (double)it + log_s);
+        if (a.out_lse) a.out_lse[row] = lp_lse(st, log_s, it);
         if (a.out_rows) a.out_rows[row] = {st.m, st.s, h, it};
     }
+    if (cl > 1) cluster_wait();
 }
+static_assert(kLpMaxIds <= 256, "a thread per given id");
 
 // ---- gradient ----
 struct LpBackArgs {
@@ -560,7 +851,7 @@ __global__ void __launch_bounds__(kLpBackThreads, 4) zs_logprobs_backward_kernel
     }
     const float gh = a.g_entropy ? a.g_entropy[row] : 0.0f;
     const float gz = a.g_lse ? a.g_lse[row] : 0.0f;
-    const double log_s = dead ? 0.0 : log((double)rw.sum);
+    const double log_s = dead ? 0.0 : log((double)rw.sum);  // once per CTA and row
     // p (z - g - h H - h log p) it = e (ca + cb t), log p = ln 2 t - ln s
     const float inv_s = dead ? 0.0f : 1.0f / rw.sum;
     const float ca = (float)((double)rw.inv_temp *

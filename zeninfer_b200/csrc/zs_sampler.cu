@@ -371,7 +371,6 @@ struct zs_context {
     int32_t lm_tiles = ZS_LMHEAD_TILES_AUTO;  // zs_set_lmhead_tiles
     int lm_pairs = 0;                         // resident CTA pairs of zs_lmhead_kernel<2>
     int32_t spec_mode = ZS_SPECULATION_ON;    // zs_set_speculation
-    int lp_max_cl = 8;                        // CTAs per row of zs_logprobs_kernel at most
     int small_clusters = 0;                   // zs_small_kernel clusters resident at once (0: none)
     int32_t small_max_rows = 8;               // zs_set_small_batch
     std::vector<TimedLaunch> timed;      // recorded since the last zs_get_timing
@@ -820,80 +819,31 @@ zs_status wait_collectives(zs_context* h, void* comm, cudaStream_t st, Clock::ti
 // ---- log probabilities and the embedding table: launches ----
 namespace {
 
-template <typename T, int NT, bool TOP>
-cudaError_t setup_logprobs(int* max_cl) {
-    auto k = zs::zs_logprobs_kernel<T, NT, TOP>;
-    cudaError_t e = cudaSuccess;
-    if (TOP)
-        e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 (int)sizeof(zs::LpTopSmem<NT>));
-    if (e != cudaSuccess) return e;
-    // 16 CTAs per row is a non-portable cluster size; where it is refused or cannot be
-    // resident, 8 are used
-    bool ok = cudaFuncSetAttribute(k, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess;
-    if (ok) {
-        cudaLaunchAttribute attr[1];
-        attr[0].id = cudaLaunchAttributeClusterDimension;
-        attr[0].val.clusterDim.x = zs::kLpMaxCl;
-        attr[0].val.clusterDim.y = 1;
-        attr[0].val.clusterDim.z = 1;
-        cudaLaunchConfig_t cfg;
-        std::memset(&cfg, 0, sizeof(cfg));
-        cfg.gridDim = dim3(zs::kLpMaxCl);
-        cfg.blockDim = dim3(NT);
-        cfg.dynamicSmemBytes = TOP ? sizeof(zs::LpTopSmem<NT>) : 0;
-        cfg.attrs = attr;
-        cfg.numAttrs = 1;
-        int n = 0;
-        ok = cudaOccupancyMaxActiveClusters(&n, k, &cfg) == cudaSuccess && n > 0;
-    }
-    (void)cudaGetLastError();
-    if (!ok) *max_cl = std::min(*max_cl, 8);
-    return cudaSuccess;
-}
-
-template <typename T>
-cudaError_t setup_logprobs_type(int* max_cl) {
-    cudaError_t e = setup_logprobs<T, 256, true>(max_cl);
-    if (e == cudaSuccess) e = setup_logprobs<T, 256, false>(max_cl);
-    if (e == cudaSuccess) e = setup_logprobs<T, 1024, true>(max_cl);
-    if (e == cudaSuccess) e = setup_logprobs<T, 1024, false>(max_cl);
-    return e;
-}
-
-cudaError_t setup_vocab_ops(int* max_cl) {
-    *max_cl = zs::kLpMaxCl;
-    cudaError_t e = setup_logprobs_type<float>(max_cl);
-    if (e == cudaSuccess) e = setup_logprobs_type<__half>(max_cl);
-    if (e == cudaSuccess) e = setup_logprobs_type<__nv_bfloat16>(max_cl);
-    if (e == cudaSuccess)
-        e = cudaFuncSetAttribute(zs::zs_embed_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 (int)sizeof(zs::EsSmem));
-    return e;
-}
-
 int dtype_size(int32_t dtype) {
     return dtype == ZS_DTYPE_F32 ? 4 : (dtype == ZS_DTYPE_F16 || dtype == ZS_DTYPE_BF16) ? 2 : 0;
 }
 
 bool misaligned(const void* p, uintptr_t a) { return ((uintptr_t)p & (a - 1)) != 0; }
 
-// CTAs per row of zs_logprobs_kernel, and the threads of each.
+// CTAs per row of zs_logprobs_kernel, and the threads of each.  Measured on B200 at
+// 151,936 f32 columns (with 5 alternatives up to 64 rows, 20 above), in us:
+//   rows          1     16     64    128    256    512   4096
+//   256 x 8     10.2   10.9   17.3   36.9   67.6  127.4  946.8
+//   512 x 2     13.1   13.6   16.4   23.7   44.8   86.5  536.5
+//   512 x 1     15.6   16.8   19.8   22.5   34.0   64.2  411.6
+//   256 x 1     20.2   23.1   28.4   31.1   37.7   57.8  397.4
+// so: one row over 8 CTAs while that leaves SMs idle, then as many CTAs of 512 threads
+// as keep about one per SM, and from two rows per SM on one CTA of 256 threads per row.
 struct LpShape {
     int cl, nt;
 };
 LpShape lp_shape(const zs_context* h, int64_t batch, int64_t n, int esize) {
     const int64_t vecs = n * esize / 16;
-    LpShape s;
-    if (batch * zs::kLpMaxCl <= h->num_sms && vecs >= 4096) {
-        s.nt = 1024;
-        s.cl = h->lp_max_cl;
-    } else {
-        s.nt = 256;
-        s.cl = 1;
-        while (s.cl < h->lp_max_cl && batch * s.cl < (int64_t)h->num_sms * 8 && vecs / (2 * s.cl) >= 512)
-            s.cl *= 2;
-    }
+    LpShape s = {1, 256};
+    if (batch >= 2 * h->num_sms || vecs < 1024) return s;
+    const int64_t room = batch * zs::kLpMaxCl <= h->num_sms ? zs::kLpMaxCl : h->num_sms / batch;
+    if (room < zs::kLpMaxCl) s.nt = 512;
+    while (2 * s.cl <= room && vecs / (2 * s.cl) >= 512) s.cl *= 2;
     return s;
 }
 
@@ -909,7 +859,6 @@ zs_status launch_logprobs(zs_context* h, const zs::LpArgs& a, cudaStream_t st) {
     std::memset(&cfg, 0, sizeof(cfg));
     cfg.gridDim = dim3((unsigned)((int64_t)a.B * a.cl));
     cfg.blockDim = dim3(NT);
-    cfg.dynamicSmemBytes = TOP ? sizeof(zs::LpTopSmem<NT>) : 0;
     cfg.stream = st;
     cfg.attrs = attr;
     cfg.numAttrs = a.cl > 1 ? 1 : 0;
@@ -921,7 +870,7 @@ template <typename T>
 zs_status launch_logprobs_type(zs_context* h, const zs::LpArgs& a, int nt, cudaStream_t st) {
     if (nt == 256)
         return a.k > 0 ? launch_logprobs<T, 256, true>(h, a, st) : launch_logprobs<T, 256, false>(h, a, st);
-    return a.k > 0 ? launch_logprobs<T, 1024, true>(h, a, st) : launch_logprobs<T, 1024, false>(h, a, st);
+    return a.k > 0 ? launch_logprobs<T, 512, true>(h, a, st) : launch_logprobs<T, 512, false>(h, a, st);
 }
 
 // Checks shared by zs_logprobs and its backward pass.
@@ -1115,8 +1064,9 @@ zs_status zs_create(int device, zs_handle* out) {
          (e = cudaFuncSetAttribute(zs::zs_lmhead_kernel<2, true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                    (int)zs::kLmSmemBytes)) != cudaSuccess))
         return cleanup(cuda_fail(e, "cudaFuncSetAttribute zs_lmhead_kernel (statistics)"));
-    if ((e = setup_vocab_ops(&h->lp_max_cl)) != cudaSuccess)
-        return cleanup(cuda_fail(e, "cudaFuncSetAttribute (log probabilities, embedding)"));
+    if ((e = cudaFuncSetAttribute(zs::zs_embed_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                  (int)sizeof(zs::EsSmem))) != cudaSuccess)
+        return cleanup(cuda_fail(e, "cudaFuncSetAttribute zs_embed_sort_kernel"));
     // CTA pairs of the lm_head kernel that can be resident at once (0: none; the
     // one-CTA tiles are used then).
     h->lm_pairs = 0;

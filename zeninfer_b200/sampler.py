@@ -14,7 +14,6 @@ Torch provides device memory and streams; all compute is in libzs_sampler.so.
 
 from __future__ import annotations
 
-import contextlib
 import ctypes as C
 import threading
 from dataclasses import dataclass
@@ -90,16 +89,62 @@ class SampleResult:
     cand_probs: Optional["object"] = None  # torch float64 [B, cand_ld]
 
 
-@dataclass
 class LogprobResult:
     """Sampler.logprobs / lmhead_logprobs: torch tensors on the device, float32 unless
-    noted.  B rows, m given ids, k alternatives."""
-    logp: Optional["object"]      # [B, m] ([B] for ids [B]); None without ids
-    entropy: "object"             # [B]
-    lse: "object"                 # [B]
-    top_ids: Optional["object"] = None   # int32 [B, k]
-    top_logp: Optional["object"] = None  # [B, k]
-    rows: Optional["object"] = None      # [B, 4] max, sum, entropy, inv_temp: for the gradient
+    noted, all of them views of one buffer.  B rows, m given ids, k alternatives.
+
+        rows      [B, 4] max, sum, entropy, inv_temp: for logprobs_backward (else None)
+        logp      [B, m], or [B] for ids [B]; None without ids
+        entropy   [B]
+        lse       [B]
+        top_ids   int32 [B, k]; None without alternatives
+        top_logp  [B, k]
+    """
+
+    __slots__ = ("_buf", "_B", "_k", "_rows", "_ids_shape", "_m")
+
+    def __init__(self, buf, B, rows, ids_shape, m, k):
+        self._buf, self._B, self._rows, self._ids_shape, self._m, self._k = \
+            buf, B, rows, ids_shape, m, k
+
+    @staticmethod
+    def size(B, rows, m, k):
+        """Floats of the buffer: rows, entropy, lse, logp, top_logp, top_ids, in order."""
+        return B * ((4 if rows else 0) + 2 + m + 2 * k)
+
+    def _at(self, before):
+        return self._B * ((4 if self._rows else 0) + before)
+
+    def _view(self, before, *shape):
+        stride = (shape[1], 1) if len(shape) == 2 else (1,)
+        return self._buf.as_strided(shape, stride, self._at(before))
+
+    @property
+    def rows(self):
+        return self._buf.as_strided((self._B, 4), (4, 1), 0) if self._rows else None
+
+    @property
+    def entropy(self):
+        return self._view(0, self._B)
+
+    @property
+    def lse(self):
+        return self._view(1, self._B)
+
+    @property
+    def logp(self):
+        return None if self._ids_shape is None else self._view(2, *self._ids_shape)
+
+    @property
+    def top_logp(self):
+        return self._view(2 + self._m, self._B, self._k) if self._k else None
+
+    @property
+    def top_ids(self):
+        if not self._k:
+            return None
+        import torch
+        return self._view(2 + self._m + self._k, self._B, self._k).view(torch.int32)
 
 
 def _params_array(params, batch):
@@ -118,11 +163,6 @@ def _stream_ptr(stream):
     return C.c_void_p(stream.cuda_stream)
 
 
-def _dtype_codes():
-    import torch
-    return {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
-
-
 class Sampler:
     """Batched device sampler bound to one CUDA device (a zs_handle)."""
 
@@ -134,7 +174,11 @@ class Sampler:
                            torch.device(device).index if not isinstance(device, int) else device)
         self.device = dev
         self._lib = _native.lib()
-        self._dtypes = _dtype_codes()
+        self._torch = torch
+        self._dtypes = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+        # the current stream as an integer, without building a Stream object per call
+        self._raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+            lambda index: torch.cuda.current_stream(index).cuda_stream)
         h = C.c_void_p()
         with torch.cuda.device(dev):
             _native.check(self._lib.zs_create(dev.index, C.byref(h)), "zs_create")
@@ -351,57 +395,69 @@ class Sampler:
         return out
 
     # ---- log probabilities and the embedding table ----
-    def _stream(self, stream):
-        """(stream pointer, context that allocates on that stream) of this sampler's device."""
-        import torch
+    def _new(self, n, dtype, stream):
+        """n elements on this device, allocated for use on `stream`."""
         if stream is None:
-            return torch.cuda.current_stream(self.device).cuda_stream, contextlib.nullcontext()
-        return stream.cuda_stream, torch.cuda.stream(stream)
+            return self._torch.empty(n, dtype=dtype, device=self.device)
+        with self._torch.cuda.stream(stream):
+            return self._torch.empty(n, dtype=dtype, device=self.device)
+
+    def _on(self, stream):
+        """The stream's pointer: the given one, or this device's current one."""
+        if stream is not None:
+            return stream.cuda_stream
+        return self._raw_stream(self.device.index)
 
     def _code(self, dtype, name):
-        if dtype not in self._dtypes:
+        code = self._dtypes.get(dtype)
+        if code is None:
             raise ValueError(f"{name} must be float32, float16 or bfloat16")
-        return self._dtypes[dtype]
+        return code
 
     def _rows2d(self, t, name):
-        """t as [rows, columns] on this device with unit column stride, and its row stride."""
-        if t.dim() == 1:
-            t = t.unsqueeze(0)
-        if t.dim() != 2 or t.device != self.device:
-            raise ValueError(f"{name} must be a 2-D tensor on the sampler's device")
-        if t.shape[1] > 1 and t.stride(1) != 1:
+        """t as [rows, columns] on this device with unit column stride: rows, columns and
+        the row stride."""
+        shape = t.shape
+        if len(shape) == 2:
+            B, n = shape
+            ld, unit = t.stride()
+        elif len(shape) == 1:
+            B, n, ld, unit = 1, shape[0], shape[0], t.stride(0)
+        else:
+            raise ValueError(f"{name} must be a 2-D tensor")
+        if t.device != self.device:
+            raise ValueError(f"{name} must be on the sampler's device")
+        if unit != 1 and n > 1:
             raise ValueError(f"{name} must have unit column stride")
-        ld = t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
-        if ld < t.shape[1]:
-            raise ValueError(f"{name}'s rows must not overlap")
-        return t, ld
+        if ld < n:
+            if B > 1:
+                raise ValueError(f"{name}'s rows must not overlap")
+            ld = n
+        return B, n, ld
 
     def _given_ids(self, ids, B):
         """ids ([B] or [B, m] int32) as (pointer, row stride, m)."""
-        import torch
-        if ids is None:
-            return None, 0, 0
-        if ids.dtype != torch.int32 or ids.device != self.device or ids.dim() not in (1, 2):
+        shape = ids.shape
+        if ids.dtype != self._torch.int32 or ids.device != self.device or not 1 <= len(shape) <= 2:
             raise ValueError("ids must be int32 [B] or [B, m] on the sampler's device")
-        if ids.shape[0] != B:
+        if shape[0] != B:
             raise ValueError("ids need one row per row of logits")
-        if ids.dim() == 1:
-            m, ld, unit = 1, ids.stride(0), True
-        else:
-            m, ld, unit = ids.shape[1], ids.stride(0), ids.shape[1] <= 1 or ids.stride(1) == 1
+        m = shape[1] if len(shape) == 2 else 1
+        ld = ids.stride(0)
         if B <= 1:
             ld = max(ld, m)
-        if not unit or ld < m:
+        if ld < m or (len(shape) == 2 and m > 1 and ids.stride(1) != 1):
             raise ValueError("ids must have unit column stride and rows that do not overlap")
         return ids.data_ptr(), ld, m
 
     def _temps(self, temp, B):
         """temp (a number, or float32 [B] on the device) as (scalar, pointer)."""
-        import torch
-        if not isinstance(temp, torch.Tensor):
+        if isinstance(temp, (int, float)):
+            return temp, None
+        if not isinstance(temp, self._torch.Tensor):
             return float(temp), None
-        if temp.dtype != torch.float32 or temp.device != self.device or temp.shape != (B,) or \
-                not temp.is_contiguous():
+        if temp.dtype != self._torch.float32 or temp.device != self.device or \
+                temp.shape != (B,) or not temp.is_contiguous():
             raise ValueError("temp must be a number or a contiguous float32 [B] tensor")
         return 1.0, temp.data_ptr()
 
@@ -413,30 +469,23 @@ class Sampler:
         row's entropy and log-sum-exp.  temp: a number or float32 CUDA [B] (<= 0 counts
         as 1).  -inf logits are masked tokens; a row of them only has log p -inf and
         entropy 0.  `rows` of the result is what logprobs_backward takes."""
-        import torch
-        logits, ld = self._rows2d(logits, "logits")
-        B, V = logits.shape
+        B, V, ld = self._rows2d(logits, "logits")
         code = self._code(logits.dtype, "logits")
-        ids_ptr, ids_ld, m = self._given_ids(ids, B)
+        ids_ptr, ids_ld, m = (None, 0, 0) if ids is None else self._given_ids(ids, B)
         t, t_ptr = self._temps(temp, B)
         k = min(int(top), V)
-        st, ctx = self._stream(stream)
-        with ctx:
-            f32 = dict(dtype=torch.float32, device=self.device)
-            rows = torch.empty((B, 4), **f32)
-            stats = torch.empty((2, B), **f32)
-            logp = None if ids is None else torch.empty(ids.shape, **f32)
-            top_ids = top_logp = None
-            if k > 0:
-                top_ids = torch.empty((B, k), dtype=torch.int32, device=self.device)
-                top_logp = torch.empty((B, k), **f32)
-        p = stats.data_ptr()
-        _native.check(self._lib.zs_logprobs(
+        if k < 0 or k > _native.LOGPROBS_MAX_TOP:
+            raise ValueError(f"top must be 0 to {_native.LOGPROBS_MAX_TOP}")
+        buf = self._new(B * (6 + m + 2 * k), self._torch.float32, stream)
+        p = buf.data_ptr()
+        q = p + B * 24  # behind rows, entropy and lse
+        s = self._lib.zs_logprobs(
             self._h, logits.data_ptr(), code, ld, B, V, t, t_ptr, ids_ptr, ids_ld, m,
-            logp.data_ptr() if logp is not None else None, k if k > 0 else int(top),
-            top_ids.data_ptr() if k > 0 else None, top_logp.data_ptr() if k > 0 else None,
-            p, p + 4 * B, rows.data_ptr(), st), "zs_logprobs")
-        return LogprobResult(logp, stats[0], stats[1], top_ids, top_logp, rows)
+            q if m else None, k, q + 4 * B * (m + k) if k else None, q + 4 * B * m if k else None,
+            p + 16 * B, p + 20 * B, p, self._on(stream))
+        if s:
+            _native.check(s, "zs_logprobs")
+        return LogprobResult(buf, B, True, None if ids is None else ids.shape, m, k)
 
     def logprobs_backward(self, logits, rows, ids=None, grad_logp=None, grad_entropy=None,
                           grad_lse=None, out=None, stream=None):
@@ -445,36 +494,36 @@ class Sampler:
         `rows` of logprobs.  grad_logp has the shape of ids; grad_entropy and grad_lse
         are [B]; all float32 contiguous, each may be None.  Equal ids of a row add up.
         Returns the gradient in the logits' type (or fills `out`, which may be `logits`)."""
-        import torch
-        logits, ld = self._rows2d(logits, "logits")
-        B, V = logits.shape
+        B, V, ld = self._rows2d(logits, "logits")
         code = self._code(logits.dtype, "logits")
-        if grad_logp is None:
-            ids = None
-        elif ids is None or grad_logp.shape != ids.shape:
-            raise ValueError("grad_logp needs ids of its shape")
-        ids_ptr, ids_ld, m = self._given_ids(ids, B)
-        for g, name, shape in ((grad_logp, "grad_logp", None), (grad_entropy, "grad_entropy", (B,)),
-                               (grad_lse, "grad_lse", (B,)), (rows, "rows", (B, 4))):
-            if g is not None and (g.dtype != torch.float32 or g.device != self.device or
-                                  not g.is_contiguous() or (shape and g.shape != shape)):
+        ids_ptr, ids_ld, m = None, 0, 0
+        if grad_logp is not None:
+            if ids is None or grad_logp.shape != ids.shape:
+                raise ValueError("grad_logp needs ids of its shape")
+            ids_ptr, ids_ld, m = self._given_ids(ids, B)
+        ptrs = []
+        for g, name, shape in ((rows, "rows", (B, 4)), (grad_logp, "grad_logp", None),
+                               (grad_entropy, "grad_entropy", (B,)), (grad_lse, "grad_lse", (B,))):
+            if g is None:
+                ptrs.append(None)
+                continue
+            if g.dtype != self._torch.float32 or g.device != self.device or \
+                    not g.is_contiguous() or (shape is not None and g.shape != shape):
                 raise ValueError(f"{name} must be a contiguous float32 tensor"
                                  + (f" of shape {shape}" if shape else ""))
-        st, ctx = self._stream(stream)
+            ptrs.append(g.data_ptr())
         if out is None:
-            with ctx:
-                out = torch.empty((B, V), dtype=logits.dtype, device=self.device)
-            g2, gld = out, V
+            out = self._new((B, V), logits.dtype, stream)
+            gld = V
         else:
-            g2, gld = self._rows2d(out, "out")
-            if g2.shape != logits.shape or out.dtype != logits.dtype:
+            if out.shape != logits.shape or out.dtype != logits.dtype:
                 raise ValueError("out must have the logits' shape and type")
-        _native.check(self._lib.zs_logprobs_backward(
-            self._h, logits.data_ptr(), code, ld, B, V, rows.data_ptr(), ids_ptr, ids_ld, m,
-            grad_logp.data_ptr() if m else None,
-            grad_entropy.data_ptr() if grad_entropy is not None else None,
-            grad_lse.data_ptr() if grad_lse is not None else None, g2.data_ptr(), gld, st),
-            "zs_logprobs_backward")
+            gld = self._rows2d(out, "out")[2]
+        s = self._lib.zs_logprobs_backward(
+            self._h, logits.data_ptr(), code, ld, B, V, ptrs[0], ids_ptr, ids_ld, m,
+            ptrs[1] if m else None, ptrs[2], ptrs[3], out.data_ptr(), gld, self._on(stream))
+        if s:
+            _native.check(s, "zs_logprobs_backward")
         return out
 
     def lmhead_logprobs(self, hidden, norm_w, weight, ids=None, temp=1.0, eps: float = 1e-6,
@@ -484,35 +533,33 @@ class Sampler:
         `hidden` ([B, E] float32 CUDA; weight bfloat16 CUDA [V, E]), without the logits
         in memory.  No alternatives and no gradient (`top_*` and `rows` are None): train
         with lmhead_logits, logprobs and logprobs_backward."""
-        import torch
-        hidden, hld = self._rows2d(hidden, "hidden")
+        torch = self._torch
+        B, E, hld = self._rows2d(hidden, "hidden")
         if hidden.dtype != torch.float32:
             raise ValueError("hidden must be float32")
         if weight.dtype != torch.bfloat16 or not weight.is_contiguous() or weight.dim() != 2 or \
                 weight.device != self.device:
             raise ValueError("weight must be a contiguous bfloat16 [V, E] tensor")
-        B, E = hidden.shape
         V = weight.shape[0]
         if weight.shape[1] != E or norm_w.numel() != E or norm_w.dtype != torch.float32 or \
                 not norm_w.is_contiguous() or norm_w.device != self.device:
             raise ValueError("weight [V, E] and norm_w [E] float32 must match hidden's E")
-        ids_ptr, ids_ld, m = self._given_ids(ids, B)
+        ids_ptr, ids_ld, m = (None, 0, 0) if ids is None else self._given_ids(ids, B)
         t, t_ptr = self._temps(temp, B)
         need = C.c_int64()
-        _native.check(self._lib.zs_lmhead_logprobs_workspace(self._h, B, E, V, C.byref(need)),
-                      "zs_lmhead_logprobs_workspace")
-        st, ctx = self._stream(stream)
-        with ctx:
-            f32 = dict(dtype=torch.float32, device=self.device)
-            stats = torch.empty((2, B), **f32)
-            logp = None if ids is None else torch.empty(ids.shape, **f32)
-            ws = torch.empty(need.value, dtype=torch.uint8, device=self.device)
-        p = stats.data_ptr()
-        _native.check(self._lib.zs_lmhead_logprobs(
-            self._h, hidden.data_ptr(), hld, norm_w.data_ptr(), float(eps), weight.data_ptr(), B,
-            E, V, t, t_ptr, ids_ptr, ids_ld, m, logp.data_ptr() if m else None, p, p + 4 * B,
-            ws.data_ptr(), need.value, st), "zs_lmhead_logprobs")
-        return LogprobResult(logp, stats[0], stats[1])
+        s = self._lib.zs_lmhead_logprobs_workspace(self._h, B, E, V, C.byref(need))
+        if s:
+            _native.check(s, "zs_lmhead_logprobs_workspace")
+        buf = self._new(B * (2 + m), torch.float32, stream)
+        ws = self._new(need.value, torch.uint8, stream)
+        p = buf.data_ptr()
+        s = self._lib.zs_lmhead_logprobs(
+            self._h, hidden.data_ptr(), hld, norm_w.data_ptr(), eps, weight.data_ptr(), B,
+            E, V, t, t_ptr, ids_ptr, ids_ld, m, p + 8 * B if m else None, p, p + 4 * B,
+            ws.data_ptr(), need.value, self._on(stream))
+        if s:
+            _native.check(s, "zs_lmhead_logprobs")
+        return LogprobResult(buf, B, False, None if ids is None else ids.shape, m, 0)
 
     def embed(self, table, ids, scale: float = 1.0, out_dtype=None, out=None, stream=None):
         """scale * table[ids] for int32 CUDA `ids` of any contiguous shape: rows of `table`
@@ -520,29 +567,25 @@ class Sampler:
         id outside the table (-1: a stopped row of decode_step).  Returns ids.shape + [E]
         in out_dtype (default the table's type), or fills `out` ([n, E], unit column
         stride)."""
-        import torch
         if table.dim() != 2:
             raise ValueError("table must be [V, E]")
-        table, tld = self._rows2d(table, "table")
-        V, E = table.shape
+        V, E, tld = self._rows2d(table, "table")
         tcode = self._code(table.dtype, "table")
-        if ids.dtype != torch.int32 or ids.device != self.device or not ids.is_contiguous():
+        if ids.dtype != self._torch.int32 or ids.device != self.device or not ids.is_contiguous():
             raise ValueError("ids must be contiguous int32 on the sampler's device")
         n = ids.numel()
-        st, ctx = self._stream(stream)
         if out is None:
-            with ctx:
-                out = torch.empty((*ids.shape, E), dtype=out_dtype or table.dtype,
-                                  device=self.device)
+            out = self._new((*ids.shape, E), out_dtype or table.dtype, stream)
             old = E
         else:
-            o2, old = self._rows2d(out, "out")
-            if o2.shape != (n, E) or (out_dtype is not None and out.dtype != out_dtype):
+            rows, cols, old = self._rows2d(out, "out")
+            if (rows, cols) != (n, E) or (out_dtype is not None and out.dtype != out_dtype):
                 raise ValueError("out must be [n, E] of out_dtype")
         ocode = self._code(out.dtype, "out")
-        _native.check(self._lib.zs_embed(self._h, table.data_ptr(), tcode, tld, V, E,
-                                         ids.data_ptr(), n, float(scale), out.data_ptr(), ocode,
-                                         old, st), "zs_embed")
+        s = self._lib.zs_embed(self._h, table.data_ptr(), tcode, tld, V, E, ids.data_ptr(), n,
+                               scale, out.data_ptr(), ocode, old, self._on(stream))
+        if s:
+            _native.check(s, "zs_embed")
         return out
 
     def embed_backward(self, grad_out, ids, n_vocab: int, scale: float = 1.0, dtype=None,
@@ -552,34 +595,34 @@ class Sampler:
         ids that do not occur; ids outside the table give nothing.  f32 sums in a fixed
         order, rounded once to `dtype` (default grad_out's type).  With `out`
         ([n_vocab, E], unit column stride) fills it, or adds to it with accumulate=True."""
-        import torch
-        if ids.dtype != torch.int32 or ids.device != self.device or not ids.is_contiguous():
+        if ids.dtype != self._torch.int32 or ids.device != self.device or not ids.is_contiguous():
             raise ValueError("ids must be contiguous int32 on the sampler's device")
         n, E = ids.numel(), grad_out.shape[-1]
-        if grad_out.shape not in ((n, E), (*ids.shape, E)):
-            raise ValueError("grad_out must be ids.shape + [E], or [n, E]")
-        g2, gld = self._rows2d(grad_out if grad_out.dim() == 2 else grad_out.reshape(n, E),
-                               "grad_out")
+        if grad_out.shape != (n, E):
+            if grad_out.shape != (*ids.shape, E) or not grad_out.is_contiguous():
+                raise ValueError("grad_out must be [n, E], or contiguous ids.shape + [E]")
+            grad_out = grad_out.view(n, E)
+        gld = self._rows2d(grad_out, "grad_out")[2]
         gcode = self._code(grad_out.dtype, "grad_out")
-        n_vocab = int(n_vocab)
         if accumulate and out is None:
             raise ValueError("accumulate needs out")
         need = C.c_int64()
-        _native.check(self._lib.zs_embed_backward_workspace(n, E, C.byref(need)),
-                      "zs_embed_backward_workspace")
-        st, ctx = self._stream(stream)
-        with ctx:
-            if out is None:
-                out = torch.empty((n_vocab, E), dtype=dtype or grad_out.dtype, device=self.device)
-            ws = torch.empty(need.value, dtype=torch.uint8, device=self.device)
-        o2, old = self._rows2d(out, "out")
-        if o2.shape != (n_vocab, E) or (dtype is not None and out.dtype != dtype):
+        s = self._lib.zs_embed_backward_workspace(n, E, C.byref(need))
+        if s:
+            _native.check(s, "zs_embed_backward_workspace")
+        if out is None:
+            out = self._new((n_vocab, E), dtype or grad_out.dtype, stream)
+        ws = self._new(need.value, self._torch.uint8, stream)
+        rows, cols, old = self._rows2d(out, "out")
+        if (rows, cols) != (n_vocab, E) or (dtype is not None and out.dtype != dtype):
             raise ValueError("out must be [n_vocab, E] of dtype")
         ocode = self._code(out.dtype, "out")
-        _native.check(self._lib.zs_embed_backward(
-            self._h, g2.data_ptr(), gcode, gld, ids.data_ptr(), n, float(scale), n_vocab, E,
-            o2.data_ptr(), ocode, old, 1 if accumulate else 0, ws.data_ptr(), need.value, st),
-            "zs_embed_backward")
+        s = self._lib.zs_embed_backward(
+            self._h, grad_out.data_ptr(), gcode, gld, ids.data_ptr(), n, scale, n_vocab, E,
+            out.data_ptr(), ocode, old, 1 if accumulate else 0, ws.data_ptr(), need.value,
+            self._on(stream))
+        if s:
+            _native.check(s, "zs_embed_backward")
         return out
 
     LMHEAD_ROUTES = {"auto": 0, "fused": 1, "two_pass": 2, "exact": 3}
