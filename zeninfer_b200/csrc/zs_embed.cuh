@@ -39,22 +39,6 @@ __device__ __forceinline__ void em_load(const T* p, float (&v)[G]) {
     static_assert(G == 8 && sizeof(T) == 2, "one 16-byte load");
     lp_unpack(__ldg(reinterpret_cast<const uint4*>(p)), v, T());
 }
-// Loads from memory this kernel also writes (not the read-only path).
-template <int G, typename T>
-__device__ __forceinline__ void em_load_rw(const T* p, float (&v)[G]) {
-    if constexpr (sizeof(T) == 4) {
-#pragma unroll
-        for (int i = 0; i < G; i += 4) {
-            const float4 q = *reinterpret_cast<const float4*>(p + i);
-            v[i] = q.x;
-            v[i + 1] = q.y;
-            v[i + 2] = q.z;
-            v[i + 3] = q.w;
-        }
-    } else {
-        lp_unpack(*reinterpret_cast<const uint4*>(p), v, T());
-    }
-}
 template <int G>
 __device__ __forceinline__ void em_store(float* p, const float (&v)[G]) {
 #pragma unroll
@@ -141,116 +125,159 @@ __global__ void __launch_bounds__(kEmThreads) zs_embed_kernel(const EmArgs a) {
 }
 
 // ---- gradient: sort ----
-constexpr int kEsCl = 8;          // CTAs that sort (one portable cluster)
+constexpr int kEsMaxCl = 8;       // CTAs that sort at most: 1, or a cluster of 4 or 8
 constexpr int kEsThreads = 1024;
 constexpr int kEsWarps = kEsThreads / 32;
 constexpr int kEsMaxBins = 512;
+constexpr int kEsBlock = 4;       // items in flight per lane
 constexpr int kEsChunk = 32;      // sorted positions per CTA of the summing kernel
+constexpr uint32_t kEsZeroBytes = 32u << 10;  // one bulk store of zeros
 
 struct EsSmem {
-    uint32_t hist[kEsWarps][kEsMaxBins];
+    uint32_t hist[kEsWarps][kEsMaxBins];  // zeros, for the bulk stores of the other CTAs
     uint32_t tot[kEsMaxBins];   // this CTA's digit counts, read by the others
     uint32_t base[kEsMaxBins];
     uint32_t scan[kEsWarps];
 };
+static_assert(sizeof(uint32_t) * kEsWarps * kEsMaxBins >= kEsZeroBytes, "zeros fit the counters");
 
 struct EsArgs {
     const int32_t* ids;
     int32_t n, V;
+    int32_t sort_ctas;  // 1, or the cluster size
     int32_t digit_bits, passes;
-    uint32_t* key[2];  // ping-pong; the last pass writes [passes & 1]
-    uint32_t* pos[2];
-    // zero fill by the other clusters: zrows rows of zcols elements of zsize bytes,
+    uint2* pair[2];  // (id, position), ping-pong; the last pass writes [passes & 1]
+    // zero fill by the other CTAs: zrows rows of zcols elements of zsize bytes,
     // zld elements apart (zrows 0: none)
     uint8_t* z;
     int64_t zrows, zcols, zld;
     int32_t zsize;
 };
 
-// Zeroes bytes [0, bytes) at p (an element boundary) with the threads of `tid` of `nt`.
-__device__ __forceinline__ void es_zero(uint8_t* p, int64_t bytes, int64_t tid, int64_t nt) {
+// Zeroes bytes [0, bytes) at p (an element boundary) with the threads of one CTA.
+__device__ __forceinline__ void es_zero(uint8_t* p, int64_t bytes, int tid) {
     const int64_t head = min(bytes, (int64_t)((16u - ((uintptr_t)p & 15u)) & 15u));
     const int64_t nvec = (bytes - head) >> 4;
     const int64_t tail = bytes - head - (nvec << 4);
     uint4* v = reinterpret_cast<uint4*>(p + head);
-    const uint4 z = make_uint4(0u, 0u, 0u, 0u);
-    int64_t i = tid;
-    for (; i + 3 * nt < nvec; i += 4 * nt) {
-        __stcs(v + i, z);
-        __stcs(v + i + nt, z);
-        __stcs(v + i + 2 * nt, z);
-        __stcs(v + i + 3 * nt, z);
-    }
-    for (; i < nvec; i += nt) __stcs(v + i, z);
+    for (int64_t i = tid; i < nvec; i += kEsThreads) v[i] = make_uint4(0u, 0u, 0u, 0u);
     if (tid < head) p[tid] = 0;
     if (tid < tail) p[head + (nvec << 4) + tid] = 0;
 }
 
-// Cluster 0 sorts the n (id, position) pairs by id, stable, least significant digit
-// first; an id outside the table becomes V and sorts last.  The other clusters zero
-// the table meanwhile.  Per pass each warp counts the digits of its contiguous share;
-// a digit's place is the count of smaller digits, of earlier CTAs', of earlier warps'
-// and of earlier items of the warp (by __match_any_sync), all of them exact counts, so
-// the order is fixed.  The pairs stay in L2 between passes.
+__device__ __forceinline__ void bulk_store(void* dst, const void* src, uint32_t bytes) {
+    asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst),
+                 "r"(smem_addr(src)), "r"(bytes)
+                 : "memory");
+}
+
+// The first sort_ctas CTAs sort the n (id, position) pairs by id, stable, least
+// significant digit first; an id outside the table becomes V and sorts last.  The other
+// CTAs zero the table meanwhile, a contiguous one with 32 KB bulk stores from shared
+// memory.  Per pass each warp counts the digits of its contiguous share; a digit's place
+// is the count of smaller digits, of earlier CTAs', of earlier warps' and of earlier
+// items of the warp (by __match_any_sync), all of them exact counts, so the order is
+// fixed.  The pairs stay in L2 between passes.
 __global__ void __launch_bounds__(kEsThreads, 1) zs_embed_sort_kernel(const EsArgs a) {
     namespace cg = cooperative_groups;
-    extern __shared__ __align__(16) uint8_t es_raw[];
+    extern __shared__ __align__(128) uint8_t es_raw[];
     EsSmem& sm = *reinterpret_cast<EsSmem*>(es_raw);
     grid_dep_trigger();  // the summing kernel may be scheduled; it waits for this grid
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    if (blockIdx.x >= kEsCl) {
-        const int64_t z = blockIdx.x - kEsCl, nz = gridDim.x - kEsCl;
+    if (blockIdx.x >= a.sort_ctas) {
+        const int64_t z = blockIdx.x - a.sort_ctas, nz = gridDim.x - a.sort_ctas;
         if (a.zrows == 1) {
-            es_zero(a.z, a.zcols * a.zsize, z * kEsThreads + tid, nz * kEsThreads);
+            uint4* zero = reinterpret_cast<uint4*>(&sm.hist[0][0]);
+            for (int i = tid; i < (int)kEsZeroBytes / 16; i += kEsThreads)
+                zero[i] = make_uint4(0u, 0u, 0u, 0u);
+            fence_proxy_async_smem();
+            __syncthreads();
+            const int64_t bytes = a.zcols * a.zsize;
+            const int64_t head = min(bytes, (int64_t)((16u - ((uintptr_t)a.z & 15u)) & 15u));
+            const int64_t body = (bytes - head) >> 4 << 4;
+            if (tid == 0) {
+                for (int64_t o = z * kEsZeroBytes; o < body; o += nz * kEsZeroBytes)
+                    bulk_store(a.z + head + o, zero, (uint32_t)min((int64_t)kEsZeroBytes, body - o));
+                asm volatile("cp.async.bulk.commit_group;\n\tcp.async.bulk.wait_group 0;" ::: "memory");
+            }
+            if (z == 0 && tid < 32) {  // the unaligned ends
+                if (tid < head) a.z[tid] = 0;
+                if (tid < bytes - head - body) a.z[head + body + tid] = 0;
+            }
         } else {
             for (int64_t r = z; r < a.zrows; r += nz)
-                es_zero(a.z + r * a.zld * a.zsize, a.zcols * a.zsize, tid, kEsThreads);
+                es_zero(a.z + r * a.zld * a.zsize, a.zcols * a.zsize, tid);
         }
         return;
     }
     cg::cluster_group cluster = cg::this_cluster();
-    const int rank = (int)cluster.block_rank();
-    constexpr int kStep = kEsCl * kEsWarps * 32;
-    const int per = (int)(((int64_t)a.n + kStep - 1) / kStep) * 32;  // items per warp
+    const bool many = a.sort_ctas > 1;
+    const int rank = many ? (int)cluster.block_rank() : 0;
+    const int nctas = a.sort_ctas;
+    const int step = nctas * kEsWarps * 32;
+    const int per = (int)(((int64_t)a.n + step - 1) / step) * 32;  // items per warp
     const int64_t w0 = (int64_t)(rank * kEsWarps + warp) * per;
     const int lo = (int)min((int64_t)a.n, w0), hi = (int)min((int64_t)a.n, w0 + per);
     const int bins = 1 << a.digit_bits;
     const uint32_t mask = (uint32_t)bins - 1u;
     for (int p = 0; p < a.passes; ++p) {
         const int shift = p * a.digit_bits;
-        const uint32_t* src_k = a.key[p & 1];
-        const uint32_t* src_p = a.pos[p & 1];
-        uint32_t* dst_k = a.key[(p + 1) & 1];
-        uint32_t* dst_p = a.pos[(p + 1) & 1];
-        auto key_at = [&](int i) -> uint32_t {
-            if (p > 0) return __ldcg(src_k + i);
+        const uint2* src = a.pair[p & 1];
+        uint2* dst = a.pair[(p + 1) & 1];
+        auto pair_at = [&](int i) -> uint2 {
+            if (p > 0) return __ldcg(src + i);
             const int32_t id = a.ids[i];
-            return id < 0 || id >= a.V ? (uint32_t)a.V : (uint32_t)id;
+            return make_uint2(id < 0 || id >= a.V ? (uint32_t)a.V : (uint32_t)id, (uint32_t)i);
         };
-        for (int i = tid; i < kEsWarps * kEsMaxBins; i += kEsThreads) (&sm.hist[0][0])[i] = 0u;
-        __syncthreads();
-        for (int i = lo + lane; i < hi; i += 32)
-            atomicAdd(&sm.hist[warp][(key_at(i) >> shift) & mask], 1u);
+        // A block of kEsBlock x 32 items at a time, all of its loads in flight; the first
+        // block stays in registers between counting and placing.
+        uint2 k0[kEsBlock];
+#pragma unroll
+        for (int u = 0; u < kEsBlock; ++u) {
+            const int i = lo + u * 32 + lane;
+            k0[u] = i < hi ? pair_at(i) : make_uint2(0u, 0u);
+        }
+        for (int i = lane; i < bins; i += 32) sm.hist[warp][i] = 0u;
+        __syncwarp();
+#pragma unroll
+        for (int u = 0; u < kEsBlock; ++u)
+            if (lo + u * 32 + lane < hi) atomicAdd(&sm.hist[warp][(k0[u].x >> shift) & mask], 1u);
+        for (int i0 = lo + kEsBlock * 32; i0 < hi; i0 += kEsBlock * 32) {
+            uint32_t kb[kEsBlock];
+#pragma unroll
+            for (int u = 0; u < kEsBlock; ++u) {
+                const int i = i0 + u * 32 + lane;
+                kb[u] = i < hi ? pair_at(i).x : 0u;
+            }
+#pragma unroll
+            for (int u = 0; u < kEsBlock; ++u)
+                if (i0 + u * 32 + lane < hi) atomicAdd(&sm.hist[warp][(kb[u] >> shift) & mask], 1u);
+        }
         __syncthreads();
         // per digit: counts of earlier warps, and the CTA's total
-        uint32_t mine = 0;
+        uint32_t all = 0;
         if (tid < bins) {
-#pragma unroll 8
-            for (int w = 0; w < kEsWarps; ++w) {
-                const uint32_t h = sm.hist[w][tid];
-                sm.hist[w][tid] = mine;
-                mine += h;
-            }
-            sm.tot[tid] = mine;
-        }
-        cluster.sync();
-        uint32_t all = 0, before = 0;
-        if (tid < bins) {
+            uint32_t h[kEsWarps];
 #pragma unroll
-            for (int r = 0; r < kEsCl; ++r) {
-                const uint32_t t = cluster.map_shared_rank(&sm, r)->tot[tid];
-                before += r < rank ? t : 0u;
-                all += t;
+            for (int w = 0; w < kEsWarps; ++w) h[w] = sm.hist[w][tid];
+#pragma unroll
+            for (int w = 0; w < kEsWarps; ++w) {
+                sm.hist[w][tid] = all;
+                all += h[w];
+            }
+            if (many) sm.tot[tid] = all;
+        }
+        uint32_t before = 0;
+        if (many) {
+            cluster.sync();
+            if (tid < bins) {
+                all = 0;
+#pragma unroll
+                for (int r = 0; r < kEsMaxCl; ++r) {
+                    const uint32_t t = r < nctas ? cluster.map_shared_rank(&sm, r)->tot[tid] : 0u;
+                    before += r < rank ? t : 0u;
+                    all += t;
+                }
             }
         }
         // exclusive prefix of `all` over the digits
@@ -262,30 +289,39 @@ __global__ void __launch_bounds__(kEsThreads, 1) zs_embed_sort_kernel(const EsAr
         }
         if (lane == 31) sm.scan[warp] = inc;
         __syncthreads();
-        uint32_t off = 0;
-        for (int w = 0; w < warp; ++w) off += sm.scan[w];
+        uint32_t off = lane < warp ? sm.scan[lane] : 0u;  // digits of earlier warps
+        off = __reduce_add_sync(kFull, off);
         if (tid < bins) sm.base[tid] = off + inc - all + before;
         __syncthreads();
-        for (int i0 = lo; i0 < hi; i0 += 32) {
-            const int i = i0 + lane;
-            const bool live = i < hi;
-            const uint32_t k = live ? key_at(i) : 0u;
-            const uint32_t d = live ? (k >> shift) & mask : 0xffffffffu;
-            const unsigned same = __match_any_sync(kFull, d);
-            const int r = __popc(same & lanemask_lt());
-            uint32_t at = 0;
-            if (live) at = sm.hist[warp][d] + (uint32_t)r + sm.base[d];
-            __syncwarp();
-            if (live && r == 0) sm.hist[warp][d] += (uint32_t)__popc(same);
-            __syncwarp();
-            if (live) {
-                dst_k[at] = k;
-                dst_p[at] = p > 0 ? __ldcg(src_p + i) : (uint32_t)i;
+        for (int i0 = lo; i0 < hi; i0 += kEsBlock * 32) {
+            if (i0 > lo) {
+#pragma unroll
+                for (int u = 0; u < kEsBlock; ++u) {
+                    const int i = i0 + u * 32 + lane;
+                    k0[u] = i < hi ? pair_at(i) : make_uint2(0u, 0u);
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < kEsBlock; ++u) {
+                if (i0 + u * 32 >= hi) break;
+                const bool live = i0 + u * 32 + lane < hi;
+                const uint32_t d = live ? (k0[u].x >> shift) & mask : 0xffffffffu;
+                const unsigned same = __match_any_sync(kFull, d);
+                const int r = __popc(same & lanemask_lt());
+                uint32_t at = 0;
+                if (live) at = sm.hist[warp][d] + (uint32_t)r + sm.base[d];
+                __syncwarp();
+                if (live && r == 0) sm.hist[warp][d] += (uint32_t)__popc(same);
+                __syncwarp();
+                if (live) dst[at] = k0[u];
             }
         }
         // every CTA's pairs of this pass are written, and every CTA has read the totals
         __threadfence();
-        cluster.sync();
+        if (many)
+            cluster.sync();
+        else
+            __syncthreads();
     }
 }
 
@@ -294,8 +330,7 @@ struct EbArgs {
     const void* grad;
     int64_t grad_ld;
     int32_t n, V, E;
-    const uint32_t* key;  // sorted ids
-    const uint32_t* pos;
+    const uint2* pair;    // (id, position), sorted
     float scale;
     void* table;
     int64_t table_ld;
@@ -304,153 +339,199 @@ struct EbArgs {
     int32_t chunks;
 };
 
-template <typename TG, typename TT, bool VEC, int G>
-__device__ __forceinline__ void eb_write(const EbArgs& a, uint32_t id, int col, float (&acc)[G]) {
-    TT* p = reinterpret_cast<TT*>(a.table) + (int64_t)id * a.table_ld + col;
-    if constexpr (VEC) {
-#pragma unroll
-        for (int j = 0; j < G; ++j) acc[j] *= a.scale;
-        if (a.accumulate) {
-            float old[G];
-            em_load_rw(p, old);
-#pragma unroll
-            for (int j = 0; j < G; ++j) acc[j] += old[j];
-        }
-        em_store(p, acc);
+// Columns per thread: 16 bytes of the wider type, so that the stores are whole; the
+// loaded elements stay packed (Raw) until they are added.
+template <typename TG, typename TT, bool VEC>
+struct EbGran {
+    static constexpr int G = !VEC ? 1 : (sizeof(TG) == 4 || sizeof(TT) == 4) ? 4 : 8;
+};
+template <int BYTES>
+struct EbRaw;
+template <>
+struct EbRaw<16> {
+    using type = uint4;
+};
+template <>
+struct EbRaw<8> {
+    using type = uint2;
+};
+template <>
+struct EbRaw<4> {
+    using type = uint32_t;
+};
+template <>
+struct EbRaw<2> {
+    using type = uint16_t;
+};
+__device__ __forceinline__ void eb_unpack(const uint4& q, float (&v)[4], float) { lp_unpack(q, v, 0.0f); }
+template <typename T>
+__device__ __forceinline__ void eb_unpack(const uint4& q, float (&v)[8], T t) {
+    lp_unpack(q, v, t);
+}
+template <typename T>
+__device__ __forceinline__ void eb_unpack(const uint2& q, float (&v)[4], T) {
+    LpPair<T>::split(q.x, v[0], v[1]);
+    LpPair<T>::split(q.y, v[2], v[3]);
+}
+__device__ __forceinline__ void eb_unpack(uint32_t q, float (&v)[1], float) { v[0] = __uint_as_float(q); }
+template <typename T>
+__device__ __forceinline__ void eb_unpack(uint16_t q, float (&v)[1], T) {
+    v[0] = lp_float(*reinterpret_cast<const T*>(&q));
+}
+template <int G, typename T>
+__device__ __forceinline__ typename EbRaw<G * (int)sizeof(T)>::type eb_load(const T* p) {
+    return *reinterpret_cast<const typename EbRaw<G * (int)sizeof(T)>::type*>(p);
+}
+// G f32 values to their place in the type: 16 bytes, 8 for 4 narrow ones, or one value.
+template <int G, typename T>
+__device__ __forceinline__ void eb_store(T* p, const float (&v)[G]) {
+    if constexpr (G == 1) {
+        lp_store(p, v[0]);
+    } else if constexpr (G * sizeof(T) == 8) {
+        const float pad[8] = {v[0], v[1], v[2], v[3], 0.0f, 0.0f, 0.0f, 0.0f};
+        const uint4 q = lp_pack(pad, T());
+        *reinterpret_cast<uint2*>(p) = make_uint2(q.x, q.y);
     } else {
-        float v = acc[0] * a.scale;
-        if (a.accumulate) v += lp_float(*p);
-        lp_store(p, v);
+        em_store(p, v);
     }
 }
 
-// One CTA sums kEsChunk sorted positions, a granule of columns per thread.  A run of
-// equal ids inside the chunk is finished here; one that crosses its borders leaves a
-// partial sum for zs_embed_join_kernel.
+template <typename TT, int G>
+__device__ __forceinline__ void eb_write(const EbArgs& a, uint32_t id, int col, float (&acc)[G]) {
+    TT* p = reinterpret_cast<TT*>(a.table) + (int64_t)id * a.table_ld + col;
+#pragma unroll
+    for (int j = 0; j < G; ++j) acc[j] *= a.scale;
+    if (a.accumulate) {
+        float old[G];
+        eb_unpack(eb_load<G>(p), old, TT());
+#pragma unroll
+        for (int j = 0; j < G; ++j) acc[j] += old[j];
+    }
+    eb_store(p, acc);
+}
+
+// One CTA sums kEsChunk sorted positions, G columns per thread, with the next kAhead
+// rows loading while it adds these.  A run of equal ids inside the chunk is finished
+// here; one that crosses its borders leaves a partial sum for zs_embed_join_kernel.
+constexpr int kEbThreads = 256;
 template <typename TG, typename TT, bool VEC>
-__global__ void __launch_bounds__(128) zs_embed_sum_kernel(const EbArgs a) {
-    constexpr int G = VEC ? EmGran<TG, TT>::G : 1;
-    constexpr int kAhead = 8;  // rows in flight
+__global__ void __launch_bounds__(kEbThreads, 4) zs_embed_sum_kernel(const EbArgs a) {
+    constexpr int G = EbGran<TG, TT, VEC>::G;
+    using Raw = typename EbRaw<G * (int)sizeof(TG)>::type;
+    constexpr int kAhead = 8;
     __shared__ uint32_t keys[kEsChunk + 2];  // [0] before the chunk, then the chunk, then after
     __shared__ uint32_t poss[kEsChunk];
     grid_dep_trigger();
     grid_dep_wait();  // the sorted pairs
     const int s0 = blockIdx.x * kEsChunk;
-    const int cnt = min(kEsChunk, a.n - s0);
+    int cnt = min(kEsChunk, a.n - s0);
     const uint32_t none = 0xffffffffu;  // not an id: those are below 2^31
     for (int i = threadIdx.x; i < kEsChunk + 2; i += blockDim.x) {
         const int p = s0 + i - 1;
-        keys[i] = (p >= 0 && p < a.n) ? a.key[p] : none;
-        if (i < cnt) poss[i] = a.pos[s0 + i];
+        const uint2 q = (p >= 0 && p < a.n) ? a.pair[p] : make_uint2(none, 0u);
+        keys[i] = q.x;
+        if (i > 0 && i <= cnt) poss[i - 1] = q.y;
     }
     __syncthreads();
+    while (cnt > 0 && keys[cnt] >= (uint32_t)a.V) --cnt;  // ids outside the table sort last
     const int col = (blockIdx.y * blockDim.x + threadIdx.x) * G;
-    if (col >= a.E) return;
+    if (col >= a.E || cnt == 0) return;
     const TG* grad = reinterpret_cast<const TG*>(a.grad) + col;
     float acc[G];
 #pragma unroll
     for (int j = 0; j < G; ++j) acc[j] = 0.0f;
     bool came_in = keys[0] == keys[1];  // the current run began in an earlier chunk
-    for (int i0 = 0; i0 < cnt; i0 += kAhead) {
-        float v[kAhead][G];
+    Raw now[kAhead];
 #pragma unroll
-        for (int u = 0; u < kAhead; ++u) {
-            if (i0 + u < cnt && keys[i0 + u + 1] < (uint32_t)a.V) {
-                const TG* p = grad + (int64_t)poss[i0 + u] * a.grad_ld;
-                if constexpr (VEC)
-                    em_load(p, v[u]);
-                else
-                    v[u][0] = lp_float(*p);
-            }
-        }
+    for (int u = 0; u < kAhead; ++u)
+        if (u < cnt) now[u] = eb_load<G>(grad + (int64_t)poss[u] * a.grad_ld);
+    for (int i0 = 0; i0 < cnt; i0 += kAhead) {
+        Raw next[kAhead];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u)
+            if (i0 + kAhead + u < cnt)
+                next[u] = eb_load<G>(grad + (int64_t)poss[i0 + kAhead + u] * a.grad_ld);
 #pragma unroll
         for (int u = 0; u < kAhead; ++u) {
             const int i = i0 + u;
-            if (i >= cnt) break;
-            const uint32_t id = keys[i + 1];
-            if (id >= (uint32_t)a.V) break;  // ids outside the table sort last
+            if (i < cnt) {
+                float v[G];
+                eb_unpack(now[u], v, TG());
 #pragma unroll
-            for (int j = 0; j < G; ++j) acc[j] += v[u][j];
-            const bool ends = keys[i + 2] != id;
-            if (ends || i + 1 == cnt) {
-                if (ends && !came_in) {
-                    eb_write<TG, TT, VEC>(a, id, col, acc);
-                } else {
-                    float* p = a.part + ((int64_t)blockIdx.x * 2 + (came_in ? 0 : 1)) * a.E + col;
+                for (int j = 0; j < G; ++j) acc[j] += v[j];
+                const uint32_t id = keys[i + 1];
+                const bool ends = keys[i + 2] != id;
+                if (ends || i + 1 == cnt) {
+                    if (ends && !came_in)
+                        eb_write<TT>(a, id, col, acc);
+                    else
+                        eb_store(a.part + ((int64_t)blockIdx.x * 2 + (came_in ? 0 : 1)) * a.E + col, acc);
 #pragma unroll
-                    for (int j = 0; j < G; ++j) p[j] = acc[j];
+                    for (int j = 0; j < G; ++j) acc[j] = 0.0f;
+                    came_in = false;
                 }
-#pragma unroll
-                for (int j = 0; j < G; ++j) acc[j] = 0.0f;
-                came_in = false;
             }
         }
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) now[u] = next[u];
     }
 }
 
-// Finishes the runs that cross chunk borders: the CTA that has the chunk in which such
-// a run begins adds the run's partial sums, group y of its kEjGroups every kEjGroups-th
-// of them in order, then the groups in order.
-constexpr int kEjGroups = 8;
+// Finishes the runs that cross chunk borders, one CTA per border: where the run began in
+// the chunk before it, the run's partial sums are added, group y of kEjGroups every
+// kEjGroups-th of them in order, then the groups in order.
+constexpr int kEjGroups = 4;
 template <typename TG, typename TT, bool VEC>
-__global__ void __launch_bounds__(128 * kEjGroups) zs_embed_join_kernel(const EbArgs a) {
-    constexpr int G = VEC ? EmGran<TG, TT>::G : 1;
-    extern __shared__ float ej_part[];  // [kEjGroups][blockDim.x][G]
-    __shared__ int list[128 * kEjGroups];
-    __shared__ int nlist;
+__global__ void __launch_bounds__(kEbThreads * kEjGroups) zs_embed_join_kernel(const EbArgs a) {
+    constexpr int G = EbGran<TG, TT, VEC>::G;
+    extern __shared__ __align__(16) float ej_part[];  // [kEjGroups - 1][blockDim.x][G]
     grid_dep_wait();
+    const int64_t s1 = (int64_t)(blockIdx.x + 1) * kEsChunk, s0 = s1 - kEsChunk;  // s1 < n
+    const uint32_t k = a.pair[s1].x, last = a.pair[s1 - 1].x, first = a.pair[s0].x;
+    const uint32_t before = s0 > 0 ? a.pair[s0 - 1].x : 0xffffffffu;
+    if (k >= (uint32_t)a.V || last != k || (first == k && before == k)) return;
     const int nt = blockDim.x * blockDim.y, tid = threadIdx.y * blockDim.x + threadIdx.x;
+    // chunks whose first position belongs to the run
+    int m = 0;
+    for (;;) {
+        const int64_t at = s1 + (int64_t)(m + tid) * kEsChunk;
+        const int got = __syncthreads_count(at < a.n && a.pair[at].x == k);
+        m += got;
+        if (got < nt) break;
+    }
     const int col = (blockIdx.y * blockDim.x + threadIdx.x) * G;
-    for (int c0 = blockIdx.x; c0 < a.chunks; c0 += gridDim.x * nt) {
-        // which of this CTA's next nt chunks start a crossing run
-        if (tid == 0) nlist = 0;
-        __syncthreads();
-        const int64_t c = c0 + (int64_t)tid * gridDim.x;
-        if (c < a.chunks - 1) {
-            const int64_t s0 = c * kEsChunk, s1 = s0 + kEsChunk;  // s1 < n
-            const uint32_t k = a.key[s1];
-            const bool crosses = k < (uint32_t)a.V && a.key[s1 - 1] == k;
-            if (crosses && (a.key[s0] != k || s0 == 0 || a.key[s0 - 1] != k))
-                list[atomicAdd(&nlist, 1)] = (int)c;
-        }
-        __syncthreads();
-        const int nl = nlist;
-        for (int l = 0; l < nl; ++l) {
-            const int ch = list[l];
-            const uint32_t k = a.key[(int64_t)(ch + 1) * kEsChunk];
-            // chunks after ch whose first position belongs to the run
-            int m = 0;
-            for (;;) {
-                const int64_t at = (int64_t)(ch + 1 + m + tid) * kEsChunk;
-                const int got = __syncthreads_count(at < a.n && a.key[at] == k);
-                m += got;
-                if (got < nt) break;
-            }
-            float acc[G];
+    float acc[G];
 #pragma unroll
-            for (int j = 0; j < G; ++j) acc[j] = 0.0f;
-            if (col < a.E) {
-#pragma unroll 8
-                for (int i = threadIdx.y; i <= m; i += kEjGroups) {
-                    const float* p = a.part + ((int64_t)(ch + i) * 2 + (i == 0 ? 1 : 0)) * a.E + col;
+    for (int j = 0; j < G; ++j) acc[j] = 0.0f;
+    if (col < a.E) {
+#pragma unroll 4
+        for (int i = threadIdx.y; i <= m; i += kEjGroups) {
+            const float* p = a.part + ((int64_t)(blockIdx.x + i) * 2 + (i == 0 ? 1 : 0)) * a.E + col;
+            if constexpr (G == 1) {
+                acc[0] += *p;
+            } else {
 #pragma unroll
-                    for (int j = 0; j < G; ++j) acc[j] += p[j];
+                for (int j = 0; j < G; j += 4) {
+                    const float4 q = *reinterpret_cast<const float4*>(p + j);
+                    acc[j] += q.x;
+                    acc[j + 1] += q.y;
+                    acc[j + 2] += q.z;
+                    acc[j + 3] += q.w;
                 }
             }
-            float* mine = ej_part + ((int)threadIdx.y * blockDim.x + threadIdx.x) * G;
-#pragma unroll
-            for (int j = 0; j < G; ++j) mine[j] = acc[j];
-            __syncthreads();
-            if (threadIdx.y == 0 && col < a.E) {
-                for (int y = 1; y < kEjGroups; ++y)
-#pragma unroll
-                    for (int j = 0; j < G; ++j)
-                        acc[j] += ej_part[(y * blockDim.x + threadIdx.x) * G + j];
-                eb_write<TG, TT, VEC>(a, k, col, acc);
-            }
-            __syncthreads();
         }
-        __syncthreads();
+    }
+    if (threadIdx.y > 0) {
+        float* mine = ej_part + ((threadIdx.y - 1) * blockDim.x + threadIdx.x) * G;
+#pragma unroll
+        for (int j = 0; j < G; ++j) mine[j] = acc[j];
+    }
+    __syncthreads();
+    if (threadIdx.y == 0 && col < a.E) {
+        for (int y = 0; y < min(kEjGroups - 1, m); ++y)
+#pragma unroll
+            for (int j = 0; j < G; ++j) acc[j] += ej_part[(y * blockDim.x + threadIdx.x) * G + j];
+        eb_write<TT>(a, k, col, acc);
     }
 }
 

@@ -371,6 +371,7 @@ struct zs_context {
     int32_t lm_tiles = ZS_LMHEAD_TILES_AUTO;  // zs_set_lmhead_tiles
     int lm_pairs = 0;                         // resident CTA pairs of zs_lmhead_kernel<2>
     int32_t spec_mode = ZS_SPECULATION_ON;    // zs_set_speculation
+    int es_clusters = 2;                      // zs_embed_sort_kernel clusters of 4 resident at once
     int small_clusters = 0;                   // zs_small_kernel clusters resident at once (0: none)
     int32_t small_max_rows = 8;               // zs_set_small_batch
     std::vector<TimedLaunch> timed;      // recorded since the last zs_get_timing
@@ -944,18 +945,19 @@ struct EmbedWs {
 EmbedWs embed_ws(int64_t n, int64_t E) {
     EmbedWs w;
     w.chunks = (int)((n + zs::kEsChunk - 1) / zs::kEsChunk);
-    w.pair_bytes = (n * 4 + 255) / 256 * 256;
-    w.part_at = 4 * w.pair_bytes;
+    w.pair_bytes = (n * 8 + 255) / 256 * 256;
+    w.part_at = 2 * w.pair_bytes;
     w.total = w.part_at + ((int64_t)w.chunks * 2 * E * 4 + 255) / 256 * 256;
     return w;
 }
 
 template <typename TG, typename TT, bool VEC>
 zs_status launch_embed_sum(zs_context* h, const zs::EbArgs& a, cudaStream_t st) {
-    constexpr int G = VEC ? zs::EmGran<TG, TT>::G : 1;
+    constexpr int G = zs::EbGran<TG, TT, VEC>::G;
     const int gran = (a.E + G - 1) / G;
-    const int bx = std::min(128, (gran + 31) / 32 * 32);
-    const unsigned tiles = (unsigned)((gran + bx - 1) / bx);
+    // the fewest column tiles, and no more threads than they need
+    const int tiles = (gran + zs::kEbThreads - 1) / zs::kEbThreads;
+    const int bx = ((gran + tiles - 1) / tiles + 31) / 32 * 32;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
@@ -966,22 +968,22 @@ zs_status launch_embed_sum(zs_context* h, const zs::EbArgs& a, cudaStream_t st) 
     cfg.numAttrs = 1;
     {
         LaunchScope scope(h, -1, st);
-        cfg.gridDim = dim3((unsigned)a.chunks, tiles);
+        cfg.gridDim = dim3((unsigned)a.chunks, (unsigned)tiles);
         cfg.blockDim = dim3(bx);
         ZS_CUDA(cudaLaunchKernelEx(&cfg, zs::zs_embed_sum_kernel<TG, TT, VEC>, a));
     }
     if (a.chunks > 1) {
         LaunchScope scope(h, -1, st);
-        cfg.gridDim = dim3((unsigned)std::min(a.chunks - 1, h->num_sms), tiles);
+        cfg.gridDim = dim3((unsigned)(a.chunks - 1), (unsigned)tiles);
         cfg.blockDim = dim3(bx, zs::kEjGroups);
-        cfg.dynamicSmemBytes = (size_t)bx * zs::kEjGroups * G * sizeof(float);
+        cfg.dynamicSmemBytes = (size_t)bx * (zs::kEjGroups - 1) * G * sizeof(float);
         ZS_CUDA(cudaLaunchKernelEx(&cfg, zs::zs_embed_join_kernel<TG, TT, VEC>, a));
     }
     return ZS_OK;
 }
 template <typename TG, typename TT>
 zs_status launch_embed_sum_vec(zs_context* h, const zs::EbArgs& a, cudaStream_t st) {
-    const bool vec = a.E % zs::EmGran<TG, TT>::G == 0 && !misaligned(a.grad, 16) &&
+    const bool vec = a.E % zs::EbGran<TG, TT, true>::G == 0 && !misaligned(a.grad, 16) &&
                      !misaligned(a.table, 16) && a.grad_ld * (int64_t)sizeof(TG) % 16 == 0 &&
                      a.table_ld * (int64_t)sizeof(TT) % 16 == 0;
     return vec ? launch_embed_sum<TG, TT, true>(h, a, st) : launch_embed_sum<TG, TT, false>(h, a, st);
@@ -1067,6 +1069,24 @@ zs_status zs_create(int device, zs_handle* out) {
     if ((e = cudaFuncSetAttribute(zs::zs_embed_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                   (int)sizeof(zs::EsSmem))) != cudaSuccess)
         return cleanup(cuda_fail(e, "cudaFuncSetAttribute zs_embed_sort_kernel"));
+    {
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = 4;
+        attr[0].val.clusterDim.y = 1;
+        attr[0].val.clusterDim.z = 1;
+        cudaLaunchConfig_t cfg;
+        std::memset(&cfg, 0, sizeof(cfg));
+        cfg.gridDim = dim3(4);
+        cfg.blockDim = dim3(zs::kEsThreads);
+        cfg.dynamicSmemBytes = sizeof(zs::EsSmem);
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        int nc = 0;
+        if ((e = cudaOccupancyMaxActiveClusters(&nc, zs::zs_embed_sort_kernel, &cfg)) != cudaSuccess)
+            return cleanup(cuda_fail(e, "occupancy of zs_embed_sort_kernel"));
+        h->es_clusters = std::max(4, nc);
+    }
     // CTA pairs of the lm_head kernel that can be resident at once (0: none; the
     // one-CTA tiles are used then).
     h->lm_pairs = 0;
@@ -2092,10 +2112,7 @@ zs_status zs_embed_backward(zs_handle h, const void* grad_out, int32_t grad_dtyp
     while (bits < 31 && ((int64_t)1 << bits) <= n_vocab) ++bits;
     e.passes = (bits + 8) / 9;
     e.digit_bits = (bits + e.passes - 1) / e.passes;
-    for (int i = 0; i < 2; ++i) {
-        e.key[i] = reinterpret_cast<uint32_t*>(ws + (2 * i) * w.pair_bytes);
-        e.pos[i] = reinterpret_cast<uint32_t*>(ws + (2 * i + 1) * w.pair_bytes);
-    }
+    for (int i = 0; i < 2; ++i) e.pair[i] = reinterpret_cast<uint2*>(ws + i * w.pair_bytes);
     if (!accumulate) {
         e.z = reinterpret_cast<uint8_t*>(grad_table);
         e.zsize = ts;
@@ -2104,22 +2121,30 @@ zs_status zs_embed_backward(zs_handle h, const void* grad_out, int32_t grad_dtyp
         e.zcols = table_ld == n_embd ? (int64_t)n_vocab * n_embd : n_embd;
     }
     {
-        // one cluster sorts; the others, one CTA per remaining SM, zero the table
+        // The CTAs that sort; the others, one per SM, zero the table meanwhile.  Measured
+        // on B200 (us of a call, 32,768 tokens): table of 544 MB 176 with one CTA, 123
+        // with four, 136 with eight (clusters of eight leave 20 SMs idle); 82 MB: 127,
+        // 59, 47; accumulating (nothing to zero): 106, 45, 34.  Up to 1024 tokens one
+        // CTA does as well as a cluster (22.1 at 1001 tokens).  Four keep up with the
+        // zeroing down to about 5000 bytes per token.
         LaunchScope scope(h, -1, st);
+        const int64_t zero_bytes = e.zrows * e.zcols * ts;
+        const int cl = n_tokens <= 1024 ? 1 : zero_bytes < 5000 * n_tokens ? 8 : 4;
+        e.sort_ctas = cl;
+        const int ctas = accumulate ? cl : cl == 1 ? h->num_sms : cl * (cl == 4 ? h->es_clusters : h->es_clusters / 2);
         cudaLaunchAttribute attr[1];
         attr[0].id = cudaLaunchAttributeClusterDimension;
-        attr[0].val.clusterDim.x = zs::kEsCl;
+        attr[0].val.clusterDim.x = (unsigned)cl;
         attr[0].val.clusterDim.y = 1;
         attr[0].val.clusterDim.z = 1;
         cudaLaunchConfig_t cfg;
         std::memset(&cfg, 0, sizeof(cfg));
-        const int clusters = accumulate ? 1 : std::max(2, h->num_sms / zs::kEsCl);
-        cfg.gridDim = dim3((unsigned)(clusters * zs::kEsCl));
+        cfg.gridDim = dim3((unsigned)ctas);
         cfg.blockDim = dim3(zs::kEsThreads);
         cfg.dynamicSmemBytes = sizeof(zs::EsSmem);
         cfg.stream = st;
         cfg.attrs = attr;
-        cfg.numAttrs = 1;
+        cfg.numAttrs = cl > 1 ? 1 : 0;
         ZS_CUDA(cudaLaunchKernelEx(&cfg, zs::zs_embed_sort_kernel, e));
     }
     if (n_tokens == 0) return ZS_OK;
@@ -2130,8 +2155,7 @@ zs_status zs_embed_backward(zs_handle h, const void* grad_out, int32_t grad_dtyp
     b.n = (int32_t)n_tokens;
     b.V = n_vocab;
     b.E = n_embd;
-    b.key = e.key[e.passes & 1];
-    b.pos = e.pos[e.passes & 1];
+    b.pair = e.pair[e.passes & 1];
     b.scale = scale;
     b.table = grad_table;
     b.table_ld = table_ld;
