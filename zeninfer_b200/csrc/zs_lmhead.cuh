@@ -94,9 +94,10 @@ struct LmArgs {
     uint32_t* tau;               // optional [B] value orders shared by a row's slices
     int* status;
     int32_t pair;                // 2: zs_lmhead_kernel<2> (CTA pairs), else <1>; host only
-    // statistics instead of a shortlist (zs_lmhead_kernel<P, true>): per (row, slice)
-    // the maximum, sum of 2^t and sum of 2^t t of the slice's logits (LpStat)
-    float4* stats;               // [B][S]
+    int32_t a_rows;              // rows of a box of xn: 128, or the batch rounded up to 8
+    // statistics instead of a shortlist (zs_lmhead_kernel<P, true>): per row and CTA (or
+    // CTA pair) the maximum, sum of 2^t and sum of 2^t t of the logits it saw (LpStat)
+    float4* stats;               // [B][gridDim.x / P]
     float temp;
     const float* row_temp;
 };
@@ -336,14 +337,37 @@ __device__ __forceinline__ bool lm_wait(uint64_t* bar, uint32_t parity, volatile
 // Units [u_begin, u_end) of this CTA (of this CTA pair for P = 2, whose CTAs are
 // consecutive blocks): a contiguous share, so consecutive units of one row tile
 // (adjacent slices) meet in one CTA and share its candidate buffers.
-template <int P>
-__device__ __forceinline__ void lm_range(const LmArgs& a, int& u_begin, int& u_end) {
+//
+// STATS: a unit is one tile, and the CTAs take them in turns, row tile by row tile of
+// one column tile after the other (kLmStatTiles row tiles at most, then the next
+// ones): all of them work on a few neighbouring column tiles at any time, so the
+// weights are read from HBM once per kLmStatTiles x kRows rows.
+constexpr int kLmStatTiles = 16;
+template <int P, bool STATS>
+__device__ __forceinline__ void lm_range(const LmArgs& a, int& u_begin, int& u_end, int& u_step) {
     const int64_t c = blockIdx.x / P, n = gridDim.x / P;
-    u_begin = (int)((c * a.n_units) / n);
-    u_end = (int)(((c + 1) * a.n_units) / n);
+    if (STATS) {
+        u_begin = (int)c;
+        u_end = a.mt * a.nt;
+        u_step = (int)n;
+    } else {
+        u_begin = (int)((c * a.n_units) / n);
+        u_end = (int)(((c + 1) * a.n_units) / n);
+        u_step = 1;
+    }
 }
 
+template <bool STATS>
 __device__ __forceinline__ void lm_unit(const LmArgs& a, int u, int& m, int& s, int& t0, int& t1) {
+    if (STATS) {
+        const int g = u / (kLmStatTiles * a.nt), r = u - g * kLmStatTiles * a.nt;
+        const int gm = min(kLmStatTiles, a.mt - g * kLmStatTiles);
+        t0 = r / gm;
+        t1 = t0 + 1;
+        m = g * kLmStatTiles + (r - t0 * gm);
+        s = 0;
+        return;
+    }
     m = u / a.S;
     s = u - m * a.S;
     t0 = (int)(((int64_t)s * a.nt) / a.S);
@@ -386,6 +410,55 @@ __global__ void zs_lm_rmsnorm_kernel(const float* hidden, int64_t hld, const flo
         }
         __syncwarp();
     }
+}
+
+// The same rmsnorm for the log probabilities: a CTA sums a row's squares side by side
+// (still in double), so xn can differ from the above only where the two double sums'
+// last bits decide a rounding.
+constexpr int kLmNormThreads = 128;
+constexpr int kLmNormHeld = 8;  // values per thread in registers: rows up to 1024
+__global__ void __launch_bounds__(kLmNormThreads) zs_lm_rmsnorm_row_kernel(
+    const float* hidden, int64_t hld, const float* norm_w, float eps, int32_t E,
+    __nv_bfloat16* xn) {
+    __shared__ double part[kLmNormThreads / 32];
+    grid_dep_trigger();  // zs_lmhead_kernel may start its weight prefetch now
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const float* x = hidden + (int64_t)blockIdx.x * hld;
+    float v[kLmNormHeld], w[kLmNormHeld];
+    double sum = 0.0;
+#pragma unroll
+    for (int j = 0; j < kLmNormHeld; ++j) {
+        const int i = tid + j * kLmNormThreads;
+        v[j] = i < E ? x[i] : 0.0f;
+        w[j] = i < E ? norm_w[i] : 0.0f;
+    }
+#pragma unroll
+    for (int j = 0; j < kLmNormHeld; ++j) sum = fma((double)v[j], (double)v[j], sum);
+#pragma unroll 4
+    for (int i = tid + kLmNormHeld * kLmNormThreads; i < E; i += kLmNormThreads) {
+        const double d = (double)x[i];
+        sum = fma(d, d, sum);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(kFull, sum, o);
+    if (lane == 0) part[warp] = sum;
+    __syncthreads();
+    sum = 0.0;
+#pragma unroll
+    for (int j = 0; j < kLmNormThreads / 32; ++j) sum += part[j];
+    const double scale = 1.0 / sqrt(sum / (double)E + (double)eps);
+    __nv_bfloat16* o = xn + (int64_t)blockIdx.x * E;
+    auto normed = [&](float a, float b) {
+        return __float2bfloat16_rn(__double2float_rn(__dmul_rn(__dmul_rn((double)a, scale), (double)b)));
+    };
+#pragma unroll
+    for (int j = 0; j < kLmNormHeld; ++j) {
+        const int i = tid + j * kLmNormThreads;
+        if (i < E) o[i] = normed(v[j], w[j]);
+    }
+#pragma unroll 4
+    for (int i = tid + kLmNormHeld * kLmNormThreads; i < E; i += kLmNormThreads)
+        o[i] = normed(x[i], norm_w[i]);
 }
 
 // ---- the lm_head in f32, in the reference's own summation order (small batches) ----
@@ -769,8 +842,14 @@ __device__ __forceinline__ void lm_chunk(const uint32_t (&r)[16], int col0, int 
 // One 32-column chunk of a tile into the running statistics of this warp's 16 rows, each
 // row's columns split over a lane pair as in lm_chunk.  Columns beyond the vocabulary
 // count as -1e30: they never raise a maximum that a real column set, and 2^t is 0.
+//
+// The base of t need not be the maximum, only near enough that the sums neither overflow
+// nor lose their small ones: it is raised to the maximum when the sum passes 2^24 (each
+// lane's first chunk, then once or twice per row), which saves the maximum of most chunks.
+// NaN takes that way too, and stays NaN.
+constexpr float kLmStatLimit = 16777216.0f;
 __device__ __forceinline__ void lm_stat_chunk(const uint32_t (&r)[16], int col0, int par, int V,
-                                              float c, LpStat& st) {
+                                              float c, LpStat2& st) {
     float v[16];
 #pragma unroll
     for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(r[j]);
@@ -779,17 +858,70 @@ __device__ __forceinline__ void lm_stat_chunk(const uint32_t (&r)[16], int col0,
         for (int j = 0; j < 16; ++j)
             if (col0 + par + 2 * j >= V) v[j] = -1e30f;
     }
-    float b[8];
+    const uint64_t c2 = f2_make(c, c);
+    auto add = [&](LpStat2& a) {
+        const float base = a.m == -INFINITY ? 0.0f : a.m;
+        const uint64_t mb = f2_make(-base, -base);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) b[j] = fmaxf(v[j], v[j + 8]);
+        for (int j = 0; j < 16; j += 2) lp_add2<true>(a, v[j], v[j + 1], mb, c2);
+    };
+    if (st.m != -INFINITY) {
+        LpStat2 a = st;
+        add(a);
+        float lo, hi;
+        f2_split(a.s, lo, hi);
+        if (lo + hi <= kLmStatLimit) {
+            st = a;
+            return;
+        }
+    }
+    float m = v[0];
 #pragma unroll
-    for (int w = 4; w >= 1; w >>= 1)
-#pragma unroll
-        for (int j = 0; j < w; ++j) b[j] = fmaxf(b[j], b[j + w]);
-    if (b[0] > st.m) lp_raise(st, b[0], c);
-    const float base = st.m == -INFINITY ? 0.0f : st.m;
-#pragma unroll
-    for (int j = 0; j < 16; ++j) lp_add(st, v[j], base, c);
+    for (int j = 1; j < 16; ++j) m = fmaxf(m, v[j]);
+    if (m > st.m) lp_raise2(st, m, c);
+    add(st);
+}
+
+// The tensor cores truncate: each f32 accumulation of 16 products drops up to a step
+// towards zero, so a logit comes out short by a share that grows with E.  For sums of
+// independent terms (partial sums that grow like the square root of their length) the
+// expected share is 0.22 x 2^-24 per accumulation; measured on B200, -4.9e-8 at E = 64,
+// -7.4e-7 at 896, -3.8e-6 at 4096.  The log probabilities take it back with 1 / temp.
+__device__ __forceinline__ float lm_inv_temp(float temp, const float* row_temp, int64_t row, int E) {
+    const float it = lp_inv_temp(temp, row_temp, row);
+    return fmaf(it, 0.22f * 5.9604645e-8f * (float)(E / 16), it);
+}
+
+// The statistics of the kLmStatTiles row tiles in work, per epilogue lane: m, s and w,
+// 256 lanes apart, kLmStatFloats per row tile.
+constexpr int kLmStatFloats = 3 * 32 * kLmEpiWarps;
+static_assert(kLmStagesMax * kLmStageBytes + kLmStatTiles * kLmStatFloats * 4 <= kLmRingBytes,
+              "the statistics fit behind the deepest ring");
+__device__ __forceinline__ void lm_stat_clear(float* states) {
+    for (int i = 0; i < kLmStatTiles; ++i) {
+        states[i * kLmStatFloats] = -INFINITY;
+        states[i * kLmStatFloats + 256] = 0.0f;
+        states[i * kLmStatFloats + 512] = 0.0f;
+    }
+}
+// Joins the lane pairs of a group of row tiles, writes this CTA's statistics of its rows
+// (empty ones too) and clears them.
+template <int P>
+__device__ __forceinline__ void lm_stat_flush(const LmArgs& a, float* states, int group, int g16,
+                                              uint32_t rank, int lane) {
+    const int64_t c = blockIdx.x / P, n = gridDim.x / P;
+    for (int i = 0; i < kLmStatTiles && group * kLmStatTiles + i < a.mt; ++i) {
+        const int row = (group * kLmStatTiles + i) * LmGeom<P>::kRows + (int)rank * kLmM + g16 + lm_dp(lane);
+        const float cc = row < a.B ? lm_inv_temp(a.temp, a.row_temp, row, a.E) * kLpLog2e : 1.0f;
+        const float* at = states + i * kLmStatFloats;
+        LpStat st = {at[0], at[256], at[512]}, other;
+        other.m = __shfl_xor_sync(kFull, st.m, 2);
+        other.s = __shfl_xor_sync(kFull, st.s, 2);
+        other.w = __shfl_xor_sync(kFull, st.w, 2);
+        st = lp_merge(st, other, cc);
+        if (row < a.B && lm_par(lane) == 0) a.stats[row * n + c] = make_float4(st.m, st.s, st.w, 0.0f);
+    }
+    lm_stat_clear(states);
 }
 
 // P = 1: one CTA per tile.  P = 2: launched in clusters of two CTAs, each pair one
@@ -849,8 +981,10 @@ __global__ void __launch_bounds__(kLmThreads, 1)
         cluster_sync_all();  // both CTAs' barriers exist before either signals the other's
     tc_fence_after();
     const uint32_t tmem = sm.tmem_base;
-    int u_begin, u_end;
-    lm_range<P>(a, u_begin, u_end);
+    int u_begin, u_end, u_step;
+    lm_range<P, STATS>(a, u_begin, u_end, u_step);
+    if (STATS) grid_dep_trigger();  // zs_lm_logprob_kernel waits for this grid
+    const uint32_t a_bytes = (uint32_t)a.a_rows * kLmBK * 2;  // of a box of xn
 
     // Launched behind zs_lm_rmsnorm_kernel as a programmatic dependent: the copy
     // issuer first pulls its first weight boxes into L2 (they do not depend on the
@@ -858,9 +992,9 @@ __global__ void __launch_bounds__(kLmThreads, 1)
     // shared bounds the rmsnorm clears.
     if (warp == 0 && lane == 0 && a.prefetch > 0) {
         int left = a.prefetch;
-        for (int u = u_begin; left > 0 && u < u_end; ++u) {
+        for (int u = u_begin; left > 0 && u < u_end; u += u_step) {
             int m, s, t0, t1;
-            lm_unit(a, u, m, s, t0, t1);
+            lm_unit<STATS>(a, u, m, s, t0, t1);
             for (int t = t0; left > 0 && t < t1; ++t)
                 for (int kb = 0; left > 0 && kb < nk; ++kb, --left)
                     tma_prefetch_l2_2d(&tm_b, kb * kLmBK, t * G::kCols + (int)rank * kLmN);
@@ -874,9 +1008,9 @@ __global__ void __launch_bounds__(kLmThreads, 1)
             uint32_t stage = 0, phase = 0;
             int64_t issued = 0;
             bool ok = true;
-            for (int u = u_begin; ok && u < u_end; ++u) {
+            for (int u = u_begin; ok && u < u_end; u += u_step) {
                 int m, s, t0, t1;
-                lm_unit(a, u, m, s, t0, t1);
+                lm_unit<STATS>(a, u, m, s, t0, t1);
                 for (int t = t0; ok && t < t1; ++t) {
                     for (int kb = 0; kb < nk; ++kb) {
                         if (!lm_wait(&sm.empty[stage], phase ^ 1u, abort)) {
@@ -884,7 +1018,7 @@ __global__ void __launch_bounds__(kLmThreads, 1)
                             break;
                         }
                         if (P == 1) {
-                            mbar_arrive_expect_tx(&sm.full[stage], kLmTileABytes + kLmTileBBytes);
+                            mbar_arrive_expect_tx(&sm.full[stage], a_bytes + kLmTileBBytes);
                             tma_load_2d(tiles_a + stage * kLmTileABytes, &tm_a, kb * kLmBK,
                                         m * kLmM, &sm.full[stage]);
                             tma_load_2d(tiles_b + stage * kLmTileBBytes, &tm_b, kb * kLmBK,
@@ -894,7 +1028,7 @@ __global__ void __launch_bounds__(kLmThreads, 1)
                             // leader alone arms; the peer's copies may land first
                             if (leader)
                                 mbar_arrive_expect_tx(&sm.full[stage],
-                                                      2u * (kLmTileABytes + kLmTileBBytes));
+                                                      2u * (a_bytes + kLmTileBBytes));
                             const uint32_t bar = smem_in_cta(&sm.full[stage], 0u);
                             tma_load_2d_pair(tiles_a + stage * kLmTileABytes, &tm_a, kb * kLmBK,
                                              m * G::kRows + (int)rank * kLmM, bar);
@@ -928,9 +1062,9 @@ __global__ void __launch_bounds__(kLmThreads, 1)
         if (lane == 0 && (P == 1 || leader)) {
             uint32_t stage = 0, phase = 0, acc = 0, acc_phase = 0;
             bool ok = true;
-            for (int u = u_begin; ok && u < u_end; ++u) {
+            for (int u = u_begin; ok && u < u_end; u += u_step) {
                 int m, s, t0, t1;
-                lm_unit(a, u, m, s, t0, t1);
+                lm_unit<STATS>(a, u, m, s, t0, t1);
                 for (int t = t0; ok && t < t1; ++t) {
                     if (!lm_wait(&sm.acc_empty[acc], acc_phase ^ 1u, abort)) {
                         ok = false;
@@ -1005,15 +1139,26 @@ __global__ void __launch_bounds__(kLmThreads, 1)
         bool open = true;      // no threshold yet: every column enters
         bool x0nan = false, has0 = false;
         int stg_buf = 0;  // logits-only staging buffer of this warp (two, alternating)
-        for (int u = u_begin; ok && u < u_end; ++u) {
+        // STATS: this lane's running statistics of each row tile, behind the ring
+        float* states = reinterpret_cast<float*>(cand) + ew * 32 + lane;
+        int stat_group = 0;
+        if (STATS) lm_stat_clear(states);
+        for (int u = u_begin; ok && u < u_end; u += u_step) {
             int m, s, t0, t1;
-            lm_unit(a, u, m, s, t0, t1);
+            lm_unit<STATS>(a, u, m, s, t0, t1);
             const int row = m * G::kRows + (int)rank * kLmM + r_in;
             const bool valid = row < a.B;
             uint32_t keff = 1;
-            LpStat stat = lp_empty();
-            const float stat_c =
-                STATS && valid ? lp_inv_temp(a.temp, a.row_temp, row) * kLpLog2e : 1.0f;
+            LpStat2 stat = {-INFINITY, 0ull, 0ull};
+            float stat_c = 1.0f;
+            float* stat_at = nullptr;
+            if constexpr (STATS) {
+                const int g = m / kLmStatTiles;
+                while (stat_group < g) lm_stat_flush<P>(a, states, stat_group++, g16, rank, lane);
+                stat_at = states + (m - g * kLmStatTiles) * kLmStatFloats;
+                stat = {stat_at[0], f2_make(stat_at[256], 0.0f), f2_make(stat_at[512], 0.0f)};
+                if (valid) stat_c = lm_inv_temp(a.temp, a.row_temp, row, a.E) * kLpLog2e;
+            }
             if (!STATS && valid) {
                 const RowPlan rp = plan_row(load_params(a.row_params, a.shared, row), a.V_total,
                                             nullptr, nullptr, 0, row);
@@ -1043,6 +1188,24 @@ __global__ void __launch_bounds__(kLmThreads, 1)
                 // owner's reading, so both lanes of a row keep one threshold)
                 uint32_t g_seen = (gtau && owner) ? lm_shared_bound(gtau) : 0u;
                 g_seen = __shfl_sync(kFull, g_seen, lane & ~2);
+                if constexpr (STATS) {
+                    // two chunks' TMEM loads alternate: one in flight while the other
+                    // chunk is added (nothing reads a buffer between issue and wait)
+                    uint32_t r0[16], r1[16];
+                    __syncwarp();
+                    tc_ld16_issue(base, r0);
+#pragma unroll 1
+                    for (int c = 0; c < G::kCols / 32; c += 2) {
+                        tc_ld16_wait(r0);
+                        __syncwarp();
+                        tc_ld16_issue(base + (uint32_t)((c + 1) * 32), r1);
+                        lm_stat_chunk(r0, tcol + c * 32, par, a.V, stat_c, stat);
+                        tc_ld16_wait(r1);
+                        __syncwarp();
+                        if (c + 2 < G::kCols / 32) tc_ld16_issue(base + (uint32_t)((c + 2) * 32), r0);
+                        lm_stat_chunk(r1, tcol + (c + 1) * 32, par, a.V, stat_c, stat);
+                    }
+                } else {
                 // The next chunk's TMEM load is in flight while this chunk is
                 // processed (rb is written asynchronously between its issue and the
                 // wait; nothing reads it there).
@@ -1057,10 +1220,6 @@ __global__ void __launch_bounds__(kLmThreads, 1)
                     for (int j = 0; j < 16; ++j) ra[j] = rb[j];
                     __syncwarp();
                     if (c + 1 < G::kCols / 32) tc_ld16_issue(base + (uint32_t)((c + 1) * 32), rb);
-                    if constexpr (STATS) {
-                        lm_stat_chunk(ra, tcol + c * 32, par, a.V, stat_c, stat);
-                        continue;
-                    }
                     if (a.tma_out) {
                         // logits only: this warp's 16 rows x 32 columns go to a staging
                         // buffer in the (here unused) candidate area, in the 128-byte
@@ -1089,6 +1248,7 @@ __global__ void __launch_bounds__(kLmThreads, 1)
                     lm_chunk(ra, tcol + c * 32, par, a.V, sel, lrow, x0nan, a.select, rows, mine,
                              count, tau_ord, tau_f, open, keff, gtau, lane);
                 }
+                }
                 if (gtau) lm_adopt(g_seen, tau_ord, tau_f, open);
                 tc_fence_before();
                 __syncwarp();  // the warp's TMEM loads have all completed
@@ -1105,13 +1265,10 @@ __global__ void __launch_bounds__(kLmThreads, 1)
             }
             if (!ok) break;
             if constexpr (STATS) {
-                LpStat other;
-                other.m = __shfl_xor_sync(kFull, stat.m, 2);
-                other.s = __shfl_xor_sync(kFull, stat.s, 2);
-                other.w = __shfl_xor_sync(kFull, stat.w, 2);
-                stat = lp_merge(stat, other, stat_c);
-                if (valid && owner)
-                    a.stats[(int64_t)row * a.S + s] = make_float4(stat.m, stat.s, stat.w, 0.0f);
+                const LpStat one = lp_single(stat);
+                stat_at[0] = one.m;
+                stat_at[256] = one.s;
+                stat_at[512] = one.w;
                 continue;
             }
             if (!a.select) continue;
@@ -1138,6 +1295,9 @@ __global__ void __launch_bounds__(kLmThreads, 1)
                 for (uint32_t i = 0; i < count; ++i) keys[i] = mine[i];
             }
         }
+        if (STATS && ok)
+            while (stat_group * kLmStatTiles < a.mt)
+                lm_stat_flush<P>(a, states, stat_group++, g16, rank, lane);
         if (!ok) set_status(a.status, kStatusTimeout);
         if (a.tma_out && lane == 0) bulk_wait_all();  // stores done before the CTA exits
         __syncwarp();
@@ -1157,7 +1317,7 @@ __global__ void __launch_bounds__(kLmThreads, 1)
     }
 }
 
-// Joins a row's slices (zs_lmhead_kernel<P, true>) and takes the given ids' logits as
+// Joins a row's S partial statistics (zs_lmhead_kernel<P, true>) and takes the given ids' logits as
 // f32 dot products of xn and the id's weight row (bf16 products are exact in f32): one
 // warp per row.
 struct LmLogprobArgs {
@@ -1178,9 +1338,18 @@ constexpr int kLmLogprobWarps = 4;
 __global__ void __launch_bounds__(32 * kLmLogprobWarps) zs_lm_logprob_kernel(const LmLogprobArgs a) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int64_t row = (int64_t)blockIdx.x * kLmLogprobWarps + warp;
+    // the first id and its weight row do not depend on the kernels before this one
+    int32_t id0 = -1;
+    if (row < a.B && a.n_ids > 0) {
+        id0 = a.ids[row * a.ids_ld];
+        if (id0 >= 0 && id0 < a.V)
+            for (int i = lane * 64; i < a.E; i += 32 * 64) prefetch_l2(a.w + (int64_t)id0 * a.E + i);
+    }
+    grid_dep_wait();  // zs_lmhead_kernel (and with it the rmsnorm)
     if (row >= a.B) return;
     const float it = lp_inv_temp(a.temp, a.row_temp, row);
-    const float c = it * kLpLog2e;
+    const float it_sum = lm_inv_temp(a.temp, a.row_temp, row, a.E);  // of the sums' logits
+    const float c = it_sum * kLpLog2e;
     LpStat st = lp_empty();
     for (int s = lane; s < a.S; s += 32) {
         const float4 q = a.stats[row * a.S + s];
@@ -1190,7 +1359,7 @@ __global__ void __launch_bounds__(32 * kLmLogprobWarps) zs_lm_logprob_kernel(con
     const float log_s = lp_log_sum(st);
     const uint4* xr = reinterpret_cast<const uint4*>(a.xn + row * a.E);
     for (int j = 0; j < a.n_ids; ++j) {
-        const int32_t id = a.ids[row * a.ids_ld + j];
+        const int32_t id = j == 0 ? id0 : a.ids[row * a.ids_ld + j];
         float lp = 0.0f;
         if (id >= 0 && id < a.V) {
             const uint4* wr = reinterpret_cast<const uint4*>(a.w + (int64_t)id * a.E);
@@ -1204,14 +1373,14 @@ __global__ void __launch_bounds__(32 * kLmLogprobWarps) zs_lm_logprob_kernel(con
             }
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) dot += __shfl_xor_sync(kFull, dot, o);
-            lp = lp_value(dot, st.m, log_s, it);
+            lp = (float)((double)dot * (double)it - ((double)st.m * (double)it_sum + (double)log_s));
             if (lp > 0.0f) lp = 0.0f;  // the two summation orders differ by their roundings
         }
         if (lane == 0) a.out_logp[row * a.n_ids + j] = lp;
     }
     if (lane == 0) {
         if (a.out_entropy) a.out_entropy[row] = lp_entropy(st, log_s);
-        if (a.out_lse) a.out_lse[row] = lp_lse(st, log_s, it);
+        if (a.out_lse) a.out_lse[row] = lp_lse(st, log_s, it_sum);
     }
 }
 
