@@ -312,8 +312,8 @@ zs_status zs_logits_stats(zs_handle h, const float* logits, int64_t ld, int32_t 
 
 /* What zs_logprobs_backward needs of a row (16 bytes). */
 typedef struct zs_logprob_row {
-    float max;      /* the row's largest logit */
-    float sum;      /* sum of exp((x - max) * inv_temp); 0 when every logit is -inf */
+    float base;     /* a logit at or near the row's largest */
+    float sum;      /* sum of exp((x - base) * inv_temp); 0 when every logit is -inf */
     float entropy;
     float inv_temp; /* 1 / temp (1 for temp <= 0) */
 } zs_logprob_row;

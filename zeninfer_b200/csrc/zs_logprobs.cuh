@@ -41,7 +41,7 @@ constexpr float kLpLog2e = 1.4426950408889634f;
 constexpr double kLpLn2 = 0.6931471805599453;
 
 struct LpRow {  // zs_logprob_row
-    float max, sum, entropy, inv_temp;
+    float base, sum, entropy, inv_temp;
 };
 
 // ---- 16-byte vectors of f32, f16 or bf16 ----
@@ -308,6 +308,34 @@ __device__ __forceinline__ void lp_add2(LpStat2& a, float lo, float hi, uint64_t
     a.w = f2_fma(e2, t2, a.w);
 }
 
+// Without alternatives the base of t need not be a maximum, only near enough that the sums
+// neither overflow nor lose their small ones, and that the large terms' t stay small (t is
+// off by up to t 2^-23): it starts as the largest of the CTA's first 8 or 16 KB segments
+// and is raised when a thread's sum passes 2^24, which saves the maximum of nearly all
+// vectors; and t is clamped only once a product e t came out NaN, that is after the
+// first -inf.  4096 bf16 rows of 151,936: 201 -> 192 us.
+constexpr float kLpLazyLimit = 16777216.0f;
+template <int U>
+__device__ __forceinline__ void lp_add_plain(LpStat2& a, const uint4 (&q)[U], float c, float) {
+    const uint64_t mb = f2_make(-a.m, -a.m), c2 = f2_make(c, c);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        lp_add2<false>(a, __uint_as_float(q[u].x), __uint_as_float(q[u].y), mb, c2);
+        lp_add2<false>(a, __uint_as_float(q[u].z), __uint_as_float(q[u].w), mb, c2);
+    }
+}
+template <int U, typename T>
+__device__ __forceinline__ void lp_add_plain(LpStat2& a, const uint4 (&q)[U], float c, T) {
+    const uint64_t mb = f2_make(-a.m, -a.m), c2 = f2_make(c, c);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        float v[8];
+        lp_unpack(q[u], v, T());
+#pragma unroll
+        for (int j = 0; j < 8; j += 2) lp_add2<false>(a, v[j], v[j + 1], mb, c2);
+    }
+}
+
 // U vectors into a statistic whose maximum is at least theirs.
 template <int U>
 __device__ __forceinline__ void lp_add_vecs(LpStat2& a, const uint4 (&q)[U], float c, uint32_t,
@@ -352,7 +380,14 @@ __device__ __forceinline__ void lp_add_vecs(LpStat2& a, const uint4 (&q)[U], flo
         }
     }
 }
-__device__ __forceinline__ uint32_t lp_low(float, float, float) { return 0u; }
+// A vector with its 16-bit values clamped from below at `low`.
+__device__ __forceinline__ uint4 lp_clamp(const uint4& q, uint32_t, float) { return q; }
+template <typename T>
+__device__ __forceinline__ uint4 lp_clamp(const uint4& q, uint32_t low, T) {
+    return make_uint4(LpPair<T>::max_nan(q.x, low), LpPair<T>::max_nan(q.y, low),
+                      LpPair<T>::max_nan(q.z, low), LpPair<T>::max_nan(q.w, low));
+}
+__device__ __forceinline__ uint32_t lp_low(float, float, float) { return lp_fill(0.0f).x; }
 template <typename T>
 __device__ __forceinline__ uint32_t lp_low(float m, float c, T) {
     return LpPair<T>::down(__fsub_rd(m, 180.0f / c));  // always below m
@@ -532,6 +567,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) zs_logprobs_kernel(const LpArgs
 
     LpStat2 st2 = {-INFINITY, 0ull, 0ull};
     uint32_t low = lp_fill(T()).x;
+    bool masked = false;  // a lane that has seen -inf clamps from then on
     int pos = -1;  // first id of the vector that holds this thread's maximum
     float edge = -INFINITY;
     bool has_edge = false;
@@ -549,12 +585,37 @@ __global__ void __launch_bounds__(NT, 1024 / NT) zs_logprobs_kernel(const LpArgs
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u)
         q[u] = first + u * 32 < v1 ? lp_stream<TOP>(xv + first + u * 32) : lp_fill(T());
+    if constexpr (!TOP) {
+        float m = -INFINITY;
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) m = fmaxf(m, lp_vec_max(q[u], T()));
+        m = lp_warp_max(m);
+        if (lane == 0) warp_stat[warp].m = m;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < NT / 32; ++w) m = fmaxf(m, warp_stat[w].m);
+        st2.m = m;  // finite or +inf: the base; -inf: no token yet
+        __syncthreads();
+    }
     for (int i = first; i - lane < v1; i += NT * kUnroll) {
         uint4 next[kUnroll];
 #pragma unroll
         for (int u = 0; u < kUnroll; ++u) {
             const int j = i + NT * kUnroll + u * 32;
             next[u] = j < v1 ? lp_stream<TOP>(xv + j) : lp_fill(T());
+        }
+        if (!TOP && !masked && st2.m != -INFINITY) {
+            // the base need not be the maximum: see kLpLazyLimit
+            LpStat2 t = st2;
+            lp_add_plain(t, q, c, T());
+            const LpStat one = lp_single(t);
+            if (one.s <= kLpLazyLimit && one.w == one.w) {
+                st2 = t;
+#pragma unroll
+                for (int u = 0; u < kUnroll; ++u) q[u] = next[u];
+                continue;
+            }
+            masked = one.s <= kLpLazyLimit;  // w is NaN: there are masked tokens (or NaN)
         }
         float m = st2.m, seg = -INFINITY;
 #pragma unroll
@@ -857,11 +918,29 @@ __global__ void __launch_bounds__(kLpBackThreads, 4) zs_logprobs_backward_kernel
     const float ca = (float)((double)rw.inv_temp *
                              ((double)gz - (double)g - (double)gh * ((double)rw.entropy - log_s))) * inv_s;
     const float cb = (float)(-(double)rw.inv_temp * (double)gh * kLpLn2) * inv_s;
-    const float base = rw.max;
+    const float base = rw.base;
     auto grad_of = [&](float v) {
         const float t = lp_max_nan((v - base) * c, kLpFloor);
         return dead ? 0.0f : fast_exp2(t) * fmaf(cb, t, ca);
     };
+    const uint64_t mb = f2_make(-base, -base), c2 = f2_make(c, c), ca2 = f2_make(ca, ca),
+                   cb2 = f2_make(cb, cb);
+    const uint32_t low = dead ? lp_fill(T()).x : lp_low(base, c, T());
+    // two elements at once (not for a row of -inf only)
+    auto grad_of2 = [&](float& lo, float& hi, bool clamp) {
+        uint64_t t2 = f2_mul(f2_add(f2_make(lo, hi), mb), c2);
+        float t0, t1;
+        f2_split(t2, t0, t1);
+        if (clamp) {
+            t0 = lp_max_nan(t0, kLpFloor);
+            t1 = lp_max_nan(t1, kLpFloor);
+            t2 = f2_make(t0, t1);
+        }
+        const uint64_t g2 = f2_mul(f2_make(fast_exp2(t0), fast_exp2(t1)), f2_fma(cb2, t2, ca2));
+        f2_split(g2, lo, hi);
+    };
+    // 16-bit values are clamped in pairs at `low` where that is finite, as in the pass
+    const bool early = sizeof(T) == 2 && low != lp_fill(T()).x;
 
     // this thread's given id, read before the chunk is overwritten
     float fix = 0.0f;
@@ -895,10 +974,16 @@ __global__ void __launch_bounds__(kLpBackThreads, 4) zs_logprobs_backward_kernel
             for (int u = 0; u < kLpBackUnroll; ++u) {
                 if (i + u * NT < cut.nvec) {
                     float v[N];
-                    lp_unpack(q[u], v, T());
+                    if (early) {
+                        lp_unpack(lp_clamp(q[u], low, T()), v, T());
 #pragma unroll
-                    for (int j = 0; j < N; ++j) v[j] = grad_of(v[j]);
-                    __stcs(gv + i + u * NT, lp_pack(v, T()));
+                        for (int j = 0; j < N; j += 2) grad_of2(v[j], v[j + 1], false);
+                    } else {
+                        lp_unpack(q[u], v, T());
+#pragma unroll
+                        for (int j = 0; j < N; j += 2) grad_of2(v[j], v[j + 1], true);
+                    }
+                    __stcs(gv + i + u * NT, dead ? make_uint4(0u, 0u, 0u, 0u) : lp_pack(v, T()));
                 }
             }
         }

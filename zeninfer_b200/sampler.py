@@ -93,7 +93,7 @@ class LogprobResult:
     """Sampler.logprobs / lmhead_logprobs: torch tensors on the device, float32 unless
     noted, all of them views of one buffer.  B rows, m given ids, k alternatives.
 
-        rows      [B, 4] max, sum, entropy, inv_temp: for logprobs_backward (else None)
+        rows      [B, 4] base, sum, entropy, inv_temp: for logprobs_backward (else None)
         logp      [B, m], or [B] for ids [B]; None without ids
         entropy   [B]
         lse       [B]
