@@ -83,31 +83,46 @@ __global__ void __launch_bounds__(kEmThreads) zs_embed_kernel(const EmArgs a) {
         if (id[u] >= a.V) id[u] = -1;
     }
     const int full = a.E / G;
-    for (int g = lane; g < full; g += a.tpr) {
-        float v[U][G];
+    if constexpr (!VEC) {
+        // element by element: kCols columns of each row in flight
+        constexpr int kCols = 4;
+        for (int g = lane; g < a.E; g += kCols * a.tpr) {
+            float v[U][kCols];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
+            for (int u = 0; u < U; ++u)
 #pragma unroll
-            for (int j = 0; j < G; ++j) v[u][j] = 0.0f;
-            if (id[u] >= 0) {
-                const TI* p = table + (int64_t)id[u] * a.table_ld + (int64_t)g * G;
-                if constexpr (VEC)
-                    em_load(p, v[u]);
-                else
-                    v[u][0] = lp_float(*p);
+                for (int j = 0; j < kCols; ++j) {
+                    const int e = g + j * a.tpr;
+                    v[u][j] = id[u] >= 0 && e < a.E ? lp_float(table[(int64_t)id[u] * a.table_ld + e]) : 0.0f;
+                }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int64_t i = i0 + (int64_t)u * rows_at_once;
+#pragma unroll
+                for (int j = 0; j < kCols; ++j) {
+                    const int e = g + j * a.tpr;
+                    if (i < a.n && e < a.E)
+                        lp_store(out + i * a.out_ld + e, id[u] >= 0 ? v[u][j] * a.scale : 0.0f);
+                }
             }
         }
+    } else {
+        for (int g = lane; g < full; g += a.tpr) {
+            float v[U][G];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int64_t i = i0 + (int64_t)u * rows_at_once;
-            if (i >= a.n) continue;
-            TO* p = out + i * a.out_ld + (int64_t)g * G;
+            for (int u = 0; u < U; ++u) {
 #pragma unroll
-            for (int j = 0; j < G; ++j) v[u][j] = id[u] >= 0 ? v[u][j] * a.scale : 0.0f;
-            if constexpr (VEC)
-                em_store(p, v[u]);
-            else
-                lp_store(p, v[u][0]);
+                for (int j = 0; j < G; ++j) v[u][j] = 0.0f;
+                if (id[u] >= 0) em_load(table + (int64_t)id[u] * a.table_ld + (int64_t)g * G, v[u]);
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int64_t i = i0 + (int64_t)u * rows_at_once;
+                if (i >= a.n) continue;
+#pragma unroll
+                for (int j = 0; j < G; ++j) v[u][j] = id[u] >= 0 ? v[u][j] * a.scale : 0.0f;
+                em_store(out + i * a.out_ld + (int64_t)g * G, v[u]);
+            }
         }
     }
     if constexpr (VEC) {  // the last E mod G columns
@@ -533,6 +548,146 @@ __global__ void __launch_bounds__(kEbThreads * kEjGroups) zs_embed_join_kernel(c
             for (int j = 0; j < G; ++j) acc[j] += ej_part[(y * blockDim.x + threadIdx.x) * G + j];
         eb_write<TT>(a, k, col, acc);
     }
+}
+
+// ---- gradient: few tokens, in one launch ----
+// Up to kEwMaxTokens tokens need no sort: every CTA holds all ids in shared memory, and
+// the CTA that takes token i finds the positions of its id by comparing them all (a
+// ballot per 32), sums those rows in order if i is the first of them, and writes the
+// table row.  The rows of ids that do not occur (a bit per row) are zeroed by bulk
+// stores issued before the sums, so the two overlap.
+constexpr int kEwMaxTokens = 1024;
+constexpr int kEwMaxVocab = 1 << 19;  // the bits take 64 KB at most
+constexpr int kEwThreads = 256;
+constexpr uint32_t kEwZeroBytes = 16u << 10;
+
+struct EwArgs {
+    EbArgs b;            // pair and part unused
+    const int32_t* ids;
+    int32_t zero;        // 1: zero the rows of other ids
+    int32_t bulk;        // bulk stores: rows start and end at 16-byte boundaries
+    int32_t group;       // rows per bulk store (a power of two up to 32, 1 if not contiguous)
+};
+// ids, ballots of two tokens, zeros, bits
+__host__ __device__ constexpr size_t ew_smem_bytes(int V) {
+    return kEwMaxTokens * 4 + 2 * (kEwMaxTokens / 32) * 4 + kEwZeroBytes + ((size_t)V + 31) / 32 * 4;
+}
+
+template <typename TG, typename TT, bool VEC>
+__global__ void __launch_bounds__(kEwThreads) zs_embed_few_kernel(const EwArgs a) {
+    constexpr int G = EbGran<TG, TT, VEC>::G;
+    using Raw = typename EbRaw<G * (int)sizeof(TG)>::type;
+    extern __shared__ __align__(128) uint8_t ew_raw[];
+    uint4* zeros = reinterpret_cast<uint4*>(ew_raw);
+    int32_t* ids = reinterpret_cast<int32_t*>(ew_raw + kEwZeroBytes);
+    uint32_t* ballots = reinterpret_cast<uint32_t*>(ids + kEwMaxTokens);  // [2][kEwMaxTokens / 32]
+    uint32_t* bits = ballots + 2 * (kEwMaxTokens / 32);
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int n = a.b.n, V = a.b.V, words = (V + 31) / 32;
+    for (int i = tid; i < kEwMaxTokens; i += kEwThreads) {
+        const int32_t id = i < n ? a.ids[i] : -1;
+        ids[i] = id < 0 || id >= V ? -1 : id;
+    }
+    TT* table = reinterpret_cast<TT*>(a.b.table);
+    if (a.zero) {
+        for (int i = tid; i < words; i += kEwThreads) bits[i] = 0u;
+        for (int i = tid; i < (int)kEwZeroBytes / 16; i += kEwThreads)
+            zeros[i] = make_uint4(0u, 0u, 0u, 0u);
+        fence_proxy_async_smem();
+    }
+    __syncthreads();
+    if (a.zero) {
+        for (int i = tid; i < n; i += kEwThreads)
+            if (ids[i] >= 0) atomicOr(&bits[ids[i] >> 5], 1u << (ids[i] & 31));
+        __syncthreads();
+        const int64_t row_bytes = (int64_t)a.b.E * sizeof(TT);
+        if (a.bulk) {
+            const int groups = (V + a.group - 1) / a.group;
+            const uint32_t gmask = a.group == 32 ? ~0u : (1u << a.group) - 1u;
+            // a thread takes a group of rows: one store where none of them occurs
+            // (neighbouring groups go to different CTAs, so that all of them store)
+            for (int g = tid * gridDim.x + blockIdx.x; g < groups; g += gridDim.x * kEwThreads) {
+                const int r0 = g * a.group, nr = min(a.group, V - r0);
+                const uint32_t here = (bits[r0 >> 5] >> (r0 & 31)) & gmask;
+                for (int r = 0; r < nr; ++r) {
+                    if ((here >> r) & 1u) continue;
+                    const int cnt = here == 0u ? nr : 1;
+                    uint8_t* p = reinterpret_cast<uint8_t*>(table + (int64_t)(r0 + r) * a.b.table_ld);
+                    const int64_t bytes = row_bytes * cnt;
+                    for (int64_t o = 0; o < bytes; o += kEwZeroBytes)
+                        bulk_store(p + o, zeros, (uint32_t)min((int64_t)kEwZeroBytes, bytes - o));
+                    r += cnt - 1;
+                }
+            }
+            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+        } else {
+            for (int r = blockIdx.x * (kEwThreads / 32) + warp; r < V; r += gridDim.x * (kEwThreads / 32)) {
+                if ((bits[r >> 5] >> (r & 31)) & 1u) continue;
+                TT* p = table + (int64_t)r * a.b.table_ld;
+                for (int c = lane; c < a.b.E; c += 32) lp_store(p + c, 0.0f);
+            }
+        }
+    }
+    const int blocks = (n + 31) / 32;
+    int turn = 0;
+    for (int i = blockIdx.x; i < n; i += gridDim.x) {
+        const int32_t id = ids[i];
+        if (id < 0) continue;  // the same for the whole CTA
+        uint32_t* mine = ballots + turn * (kEwMaxTokens / 32);
+        turn ^= 1;
+        for (int b = warp; b < blocks; b += kEwThreads / 32) {
+            const uint32_t m = __ballot_sync(kFull, ids[b * 32 + lane] == id);
+            if (lane == 0) mine[b] = m;
+        }
+        // One barrier per turn: these words were read two turns ago, before the last
+        // turn's barrier.
+        __syncthreads();
+        // lane b holds the ballot of positions 32 b .. 32 b + 31
+        const uint32_t word = lane < blocks ? mine[lane] : 0u;
+        const uint32_t before = lane < i >> 5 ? ~0u : lane == i >> 5 ? (1u << (i & 31)) - 1u : 0u;
+        if (__any_sync(kFull, (word & before) != 0u)) continue;  // not its first position
+        const uint32_t some = __ballot_sync(kFull, word != 0u);
+        // every lane of a warp stays: the ballots are handed round by shuffles
+        for (int c0 = warp * 32 * G; c0 < a.b.E; c0 += kEwThreads * G) {
+            const int col = c0 + lane * G;
+            const bool live = col < a.b.E;
+            const TG* grad = reinterpret_cast<const TG*>(a.b.grad) + (live ? col : 0);
+            float acc[G];
+#pragma unroll
+            for (int j = 0; j < G; ++j) acc[j] = 0.0f;
+            constexpr int kAhead = 8;
+            uint32_t left = some, m = 0u;
+            int b = 0;
+            while ((left | m) != 0u) {
+                Raw q[kAhead];
+                int got = 0;
+#pragma unroll
+                for (int u = 0; u < kAhead; ++u) {
+                    if (m == 0u && left != 0u) {
+                        b = __ffs(left) - 1;
+                        left &= left - 1u;
+                        m = __shfl_sync(kFull, word, b);
+                    }
+                    if (m != 0u) {
+                        if (live) q[u] = eb_load<G>(grad + (int64_t)(b * 32 + __ffs(m) - 1) * a.b.grad_ld);
+                        m &= m - 1u;
+                        got = u + 1;
+                    }
+                }
+#pragma unroll
+                for (int u = 0; u < kAhead; ++u) {
+                    if (u < got && live) {
+                        float v[G];
+                        eb_unpack(q[u], v, TG());
+#pragma unroll
+                        for (int j = 0; j < G; ++j) acc[j] += v[j];
+                    }
+                }
+            }
+            if (live) eb_write<TT>(a.b, (uint32_t)id, col, acc);
+        }
+    }
+    if (a.zero && a.bulk) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
 }
 
 }  // namespace zs

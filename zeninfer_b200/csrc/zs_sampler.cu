@@ -984,18 +984,80 @@ zs_status launch_embed_sum(zs_context* h, const zs::EbArgs& a, cudaStream_t st) 
     }
     return ZS_OK;
 }
+// Sorts the pairs and zeroes the table.  The CTAs that sort; the others, one per SM, zero
+// the table meanwhile.  Measured on B200 (us of a call, 32,768 tokens): table of 544 MB
+// 176 with one CTA, 123 with four, 136 with eight (clusters of eight leave 20 SMs idle);
+// 82 MB: 127, 59, 47; accumulating (nothing to zero): 106, 45, 34.  Up to 1024 tokens one
+// CTA does as well as a cluster.  Four keep up with the zeroing down to about 5000 bytes
+// per token.
+zs_status launch_embed_sort(zs_context* h, zs::EsArgs& e, cudaStream_t st) {
+    LaunchScope scope(h, -1, st);
+    const int64_t zero_bytes = e.zrows * e.zcols * e.zsize;
+    const int cl = e.n <= 1024 ? 1 : zero_bytes < 5000 * (int64_t)e.n ? 8 : 4;
+    e.sort_ctas = cl;
+    const int ctas = e.zrows == 0 ? cl
+                     : cl == 1    ? h->num_sms
+                                  : cl * (cl == 4 ? h->es_clusters : h->es_clusters / 2);
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)cl;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg;
+    std::memset(&cfg, 0, sizeof(cfg));
+    cfg.gridDim = dim3((unsigned)ctas);
+    cfg.blockDim = dim3(zs::kEsThreads);
+    cfg.dynamicSmemBytes = sizeof(zs::EsSmem);
+    cfg.stream = st;
+    cfg.attrs = attr;
+    cfg.numAttrs = cl > 1 ? 1 : 0;
+    ZS_CUDA(cudaLaunchKernelEx(&cfg, zs::zs_embed_sort_kernel, e));
+    return ZS_OK;
+}
+
+// Few tokens: one launch, two CTAs per SM.
+template <typename TG, typename TT, bool VEC>
+zs_status launch_embed_few(zs_context* h, const zs::EbArgs& b, const int32_t* ids, cudaStream_t st) {
+    auto k = zs::zs_embed_few_kernel<TG, TT, VEC>;
+    const size_t smem = zs::ew_smem_bytes(b.V);
+    ZS_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 (int)zs::ew_smem_bytes(zs::kEwMaxVocab)));
+    zs::EwArgs a;
+    a.b = b;
+    a.ids = ids;
+    a.zero = !b.accumulate;
+    const int64_t row = (int64_t)b.E * sizeof(TT);
+    a.bulk = !misaligned(b.table, 16) && row % 16 == 0 && b.table_ld * (int64_t)sizeof(TT) % 16 == 0;
+    a.group = 1;
+    if (b.table_ld == b.E)
+        while (a.group < 32 && 2 * a.group * row <= (int64_t)zs::kEwZeroBytes) a.group *= 2;
+    LaunchScope scope(h, -1, st);
+    const int ctas = a.zero ? 2 * h->num_sms : std::min(b.n, 2 * h->num_sms);
+    k<<<ctas, zs::kEwThreads, smem, st>>>(a);
+    ZS_CUDA(cudaGetLastError());
+    return ZS_OK;
+}
+
+template <typename TG, typename TT, bool VEC>
+zs_status launch_embed_back(zs_context* h, const zs::EbArgs& a, const int32_t* few_ids, cudaStream_t st) {
+    return few_ids ? launch_embed_few<TG, TT, VEC>(h, a, few_ids, st)
+                   : launch_embed_sum<TG, TT, VEC>(h, a, st);
+}
 template <typename TG, typename TT>
-zs_status launch_embed_sum_vec(zs_context* h, const zs::EbArgs& a, cudaStream_t st) {
+zs_status launch_embed_sum_vec(zs_context* h, const zs::EbArgs& a, const int32_t* few_ids, cudaStream_t st) {
     const bool vec = a.E % zs::EbGran<TG, TT, true>::G == 0 && !misaligned(a.grad, 16) &&
                      !misaligned(a.table, 16) && a.grad_ld * (int64_t)sizeof(TG) % 16 == 0 &&
                      a.table_ld * (int64_t)sizeof(TT) % 16 == 0;
-    return vec ? launch_embed_sum<TG, TT, true>(h, a, st) : launch_embed_sum<TG, TT, false>(h, a, st);
+    return vec ? launch_embed_back<TG, TT, true>(h, a, few_ids, st)
+               : launch_embed_back<TG, TT, false>(h, a, few_ids, st);
 }
+// few_ids: the ids for launch_embed_few, or null for the sorted way.
 template <typename TG>
-zs_status launch_embed_sum_in(zs_context* h, const zs::EbArgs& a, int32_t table_dtype, cudaStream_t st) {
-    if (table_dtype == ZS_DTYPE_F32) return launch_embed_sum_vec<TG, float>(h, a, st);
-    if (table_dtype == ZS_DTYPE_F16) return launch_embed_sum_vec<TG, __half>(h, a, st);
-    return launch_embed_sum_vec<TG, __nv_bfloat16>(h, a, st);
+zs_status launch_embed_sum_in(zs_context* h, const zs::EbArgs& a, const int32_t* few_ids,
+                              int32_t table_dtype, cudaStream_t st) {
+    if (table_dtype == ZS_DTYPE_F32) return launch_embed_sum_vec<TG, float>(h, a, few_ids, st);
+    if (table_dtype == ZS_DTYPE_F16) return launch_embed_sum_vec<TG, __half>(h, a, few_ids, st);
+    return launch_embed_sum_vec<TG, __nv_bfloat16>(h, a, few_ids, st);
 }
 
 }  // namespace
@@ -2143,52 +2205,6 @@ zs_status zs_embed_backward(zs_handle h, const void* grad_out, int32_t grad_dtyp
     cudaStream_t st = (cudaStream_t)stream;
     const EmbedWs w = embed_ws(n_tokens, n_embd);
     uint8_t* ws = reinterpret_cast<uint8_t*>(workspace);
-    zs::EsArgs e;
-    std::memset(&e, 0, sizeof(e));
-    e.ids = ids;
-    e.n = (int32_t)n_tokens;
-    e.V = n_vocab;
-    // keys 0 .. n_vocab (the last for ids outside the table)
-    int bits = 1;
-    while (bits < 31 && ((int64_t)1 << bits) <= n_vocab) ++bits;
-    e.passes = (bits + 8) / 9;
-    e.digit_bits = (bits + e.passes - 1) / e.passes;
-    for (int i = 0; i < 2; ++i) e.pair[i] = reinterpret_cast<uint2*>(ws + i * w.pair_bytes);
-    if (!accumulate) {
-        e.z = reinterpret_cast<uint8_t*>(grad_table);
-        e.zsize = ts;
-        e.zld = table_ld;
-        e.zrows = table_ld == n_embd ? 1 : n_vocab;
-        e.zcols = table_ld == n_embd ? (int64_t)n_vocab * n_embd : n_embd;
-    }
-    {
-        // The CTAs that sort; the others, one per SM, zero the table meanwhile.  Measured
-        // on B200 (us of a call, 32,768 tokens): table of 544 MB 176 with one CTA, 123
-        // with four, 136 with eight (clusters of eight leave 20 SMs idle); 82 MB: 127,
-        // 59, 47; accumulating (nothing to zero): 106, 45, 34.  Up to 1024 tokens one
-        // CTA does as well as a cluster (22.1 at 1001 tokens).  Four keep up with the
-        // zeroing down to about 5000 bytes per token.
-        LaunchScope scope(h, -1, st);
-        const int64_t zero_bytes = e.zrows * e.zcols * ts;
-        const int cl = n_tokens <= 1024 ? 1 : zero_bytes < 5000 * n_tokens ? 8 : 4;
-        e.sort_ctas = cl;
-        const int ctas = accumulate ? cl : cl == 1 ? h->num_sms : cl * (cl == 4 ? h->es_clusters : h->es_clusters / 2);
-        cudaLaunchAttribute attr[1];
-        attr[0].id = cudaLaunchAttributeClusterDimension;
-        attr[0].val.clusterDim.x = (unsigned)cl;
-        attr[0].val.clusterDim.y = 1;
-        attr[0].val.clusterDim.z = 1;
-        cudaLaunchConfig_t cfg;
-        std::memset(&cfg, 0, sizeof(cfg));
-        cfg.gridDim = dim3((unsigned)ctas);
-        cfg.blockDim = dim3(zs::kEsThreads);
-        cfg.dynamicSmemBytes = sizeof(zs::EsSmem);
-        cfg.stream = st;
-        cfg.attrs = attr;
-        cfg.numAttrs = cl > 1 ? 1 : 0;
-        ZS_CUDA(cudaLaunchKernelEx(&cfg, zs::zs_embed_sort_kernel, e));
-    }
-    if (n_tokens == 0) return ZS_OK;
     zs::EbArgs b;
     std::memset(&b, 0, sizeof(b));
     b.grad = grad_out;
@@ -2196,16 +2212,42 @@ zs_status zs_embed_backward(zs_handle h, const void* grad_out, int32_t grad_dtyp
     b.n = (int32_t)n_tokens;
     b.V = n_vocab;
     b.E = n_embd;
-    b.pair = e.pair[e.passes & 1];
     b.scale = scale;
     b.table = grad_table;
     b.table_ld = table_ld;
     b.accumulate = accumulate != 0;
-    b.part = reinterpret_cast<float*>(ws + w.part_at);
     b.chunks = w.chunks;
-    if (grad_dtype == ZS_DTYPE_F32) return launch_embed_sum_in<float>(h, b, table_dtype, st);
-    if (grad_dtype == ZS_DTYPE_F16) return launch_embed_sum_in<__half>(h, b, table_dtype, st);
-    return launch_embed_sum_in<__nv_bfloat16>(h, b, table_dtype, st);
+    const int32_t none = 0;
+    const int32_t* few = nullptr;
+    if (n_tokens <= zs::kEwMaxTokens && n_vocab <= zs::kEwMaxVocab) {
+        few = n_tokens > 0 ? ids : &none;  // not read when there are no tokens
+    } else {
+        zs::EsArgs e;
+        std::memset(&e, 0, sizeof(e));
+        e.ids = ids;
+        e.n = (int32_t)n_tokens;
+        e.V = n_vocab;
+        // keys 0 .. n_vocab (the last for ids outside the table)
+        int bits = 1;
+        while (bits < 31 && ((int64_t)1 << bits) <= n_vocab) ++bits;
+        e.passes = (bits + 8) / 9;
+        e.digit_bits = (bits + e.passes - 1) / e.passes;
+        for (int i = 0; i < 2; ++i) e.pair[i] = reinterpret_cast<uint2*>(ws + i * w.pair_bytes);
+        if (!accumulate) {
+            e.z = reinterpret_cast<uint8_t*>(grad_table);
+            e.zsize = ts;
+            e.zld = table_ld;
+            e.zrows = table_ld == n_embd ? 1 : n_vocab;
+            e.zcols = table_ld == n_embd ? (int64_t)n_vocab * n_embd : n_embd;
+        }
+        zs_status s = launch_embed_sort(h, e, st);
+        if (s != ZS_OK || n_tokens == 0) return s;
+        b.pair = e.pair[e.passes & 1];
+        b.part = reinterpret_cast<float*>(ws + w.part_at);
+    }
+    if (grad_dtype == ZS_DTYPE_F32) return launch_embed_sum_in<float>(h, b, few, table_dtype, st);
+    if (grad_dtype == ZS_DTYPE_F16) return launch_embed_sum_in<__half>(h, b, few, table_dtype, st);
+    return launch_embed_sum_in<__nv_bfloat16>(h, b, few, table_dtype, st);
 }
 
 zs_status zs_shard_partial_bytes(int32_t batch, int32_t n_vocab_total, int32_t n_ranks,
