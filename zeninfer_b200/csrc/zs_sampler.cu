@@ -909,35 +909,30 @@ cudaError_t launch_lp_backward(const zs::LpBackArgs& base, cudaStream_t st) {
     return cudaGetLastError();
 }
 
-template <typename TI, typename TO, bool VEC>
-cudaError_t launch_embed(const zs_context* h, zs::EmArgs a, cudaStream_t st) {
-    constexpr int G = VEC ? zs::EmGran<TI, TO>::G : 1;
-    const int gran = std::max(1, a.E / G);
-    a.tpr = 32;
-    while (a.tpr < zs::kEmThreads && a.tpr < gran) a.tpr *= 2;
-    const int at_once = zs::kEmThreads / a.tpr;
-    // four rows per thread once that still gives every SM several CTAs
-    if (a.n >= (int64_t)h->num_sms * 8 * at_once * 4) {
-        const int64_t grid = (a.n + at_once * 4 - 1) / (at_once * 4);
-        zs::zs_embed_kernel<TI, TO, 4, VEC><<<(unsigned)grid, zs::kEmThreads, 0, st>>>(a);
-    } else {
-        const int64_t grid = (a.n + at_once - 1) / at_once;
-        zs::zs_embed_kernel<TI, TO, 1, VEC><<<(unsigned)grid, zs::kEmThreads, 0, st>>>(a);
-    }
-    return cudaGetLastError();
-}
 template <typename TI, typename TO>
-cudaError_t launch_embed_vec(const zs_context* h, const zs::EmArgs& a, cudaStream_t st) {
+cudaError_t launch_embed(zs::EmArgs a, cudaStream_t st) {
     const bool vec = !misaligned(a.table, 16) && !misaligned(a.out, 16) &&
                      a.table_ld * (int64_t)sizeof(TI) % 16 == 0 &&
                      a.out_ld * (int64_t)sizeof(TO) % 16 == 0;
-    return vec ? launch_embed<TI, TO, true>(h, a, st) : launch_embed<TI, TO, false>(h, a, st);
+    // up to about 1000 rows a row is spread over more threads (measured: 256 rows 2.4
+    // against 2.8 us, 4096 rows 5.9 against 5.0)
+    if (!vec || a.n > 1024) {
+        const int64_t grid = (a.n + zs::kEmThreads / 32 - 1) / (zs::kEmThreads / 32);
+        zs::zs_embed_any_kernel<TI, TO><<<(unsigned)grid, zs::kEmThreads, 0, st>>>(a);
+    } else {
+        const int gran = a.E / zs::EmGran<TI, TO>::G;
+        a.tpr = 32;
+        while (a.tpr < zs::kEmThreads && a.tpr < gran) a.tpr *= 2;
+        const int rows = zs::kEmThreads / a.tpr;
+        zs::zs_embed_kernel<TI, TO><<<(unsigned)((a.n + rows - 1) / rows), zs::kEmThreads, 0, st>>>(a);
+    }
+    return cudaGetLastError();
 }
 template <typename TI>
-cudaError_t launch_embed_in(const zs_context* h, const zs::EmArgs& a, int32_t out_dtype, cudaStream_t st) {
-    if (out_dtype == ZS_DTYPE_F32) return launch_embed_vec<TI, float>(h, a, st);
-    if (out_dtype == ZS_DTYPE_F16) return launch_embed_vec<TI, __half>(h, a, st);
-    return launch_embed_vec<TI, __nv_bfloat16>(h, a, st);
+cudaError_t launch_embed_in(const zs::EmArgs& a, int32_t out_dtype, cudaStream_t st) {
+    if (out_dtype == ZS_DTYPE_F32) return launch_embed<TI, float>(a, st);
+    if (out_dtype == ZS_DTYPE_F16) return launch_embed<TI, __half>(a, st);
+    return launch_embed<TI, __nv_bfloat16>(a, st);
 }
 
 // Where the pairs and partial sums of zs_embed_backward lie in its workspace.
@@ -2154,9 +2149,9 @@ zs_status zs_embed(zs_handle h, const void* table, int32_t table_dtype, int64_t 
     a.out_ld = out_ld;
     cudaStream_t st = (cudaStream_t)stream;
     LaunchScope scope(h, -1, st);
-    ZS_CUDA(table_dtype == ZS_DTYPE_F32   ? launch_embed_in<float>(h, a, out_dtype, st)
-            : table_dtype == ZS_DTYPE_F16 ? launch_embed_in<__half>(h, a, out_dtype, st)
-                                          : launch_embed_in<__nv_bfloat16>(h, a, out_dtype, st));
+    ZS_CUDA(table_dtype == ZS_DTYPE_F32   ? launch_embed_in<float>(a, out_dtype, st)
+            : table_dtype == ZS_DTYPE_F16 ? launch_embed_in<__half>(a, out_dtype, st)
+                                          : launch_embed_in<__nv_bfloat16>(a, out_dtype, st));
     return ZS_OK;
 }
 
