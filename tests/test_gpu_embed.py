@@ -144,6 +144,24 @@ def test_embed_backward_runs(sampler, kind, n):
     assert torch.equal(sampler.embed_backward(grad, ids, V), want)
 
 
+@pytest.mark.parametrize("td", TYPES)
+@pytest.mark.parametrize("n", [0, 3, 1024, 1025])
+@pytest.mark.parametrize("V,E", [(5000, 33), (4999, 32), (100, 2049), (37, 9000), (9, 1), (4001, 6)])
+def test_embed_backward_zeroes_the_rest(sampler, td, n, V, E):
+    """Rows that no token names are zero whatever was there, in tables whose rows do and do
+    not start at 16-byte boundaries, contiguous or not; nothing else is touched."""
+    ids = ids_of(n, V, seed=5)
+    grad = torch.ones(n, E, device="cuda")
+    want = exact_grad(grad, ids, V, 1.0)[0].to(td)  # whole numbers: exact up to the rounding
+    for off, ld in ((0, E), (1, E), (0, E + 1), (0, E + 8 - E % 8)):
+        buf = torch.full((off + V * ld + 64,), 5.0, device="cuda", dtype=td)
+        view = torch.as_strided(buf, (V, E), (ld, 1), off)
+        sampler.embed_backward(grad, ids, V, out=view)
+        assert torch.equal(view, want)
+        view.fill_(5.0)
+        assert (buf == 5.0).all()  # nothing else was touched (an id may occur five times)
+
+
 def test_embed_backward_strides_streams_and_graphs(sampler):
     n, V, E = 700, 90, 40
     g = torch.Generator(device="cuda").manual_seed(4)

@@ -126,6 +126,25 @@ def test_logprobs(sampler, dtype, B, V, off, ld, m, top):
     check(sampler, rand(B, V, dtype, off=off, ld=ld), some_ids(B, V, m), 0.7, top)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("V", [129, 520, 1030, 3000, 8200])
+def test_many_alternatives_of_short_rows(sampler, dtype, V):
+    """Fewer vectors than, or about as many as, threads and alternatives."""
+    for off in (0, 3):
+        check(sampler, rand(3, V, dtype, seed=V, off=off), None, 1.0, 128)
+
+
+def test_rows_longer_than_the_kept_segments(sampler):
+    """Slices of more than 2 MB, whose segments' maxima are not kept."""
+    check(sampler, rand(1, 5_000_003, torch.float32, seed=1), some_ids(1, 5_000_003, 1), 1.0, 3)
+    x = rand(300, 700_001, torch.bfloat16, seed=2)
+    r = sampler.logprobs(x, top=2)
+    assert torch.equal(r.top_ids[::60].long(), order(x[::60], 2).to(x.device))
+    y = rand(300, 1_100_001, torch.bfloat16, seed=3)
+    r = sampler.logprobs(y, top=2)
+    assert torch.equal(r.top_ids[::100].long(), order(y[::100], 2).to(x.device))
+
+
 def test_logprobs_qwen_vocabulary(sampler):
     for B, dtype in ((1, torch.float32), (3, torch.bfloat16), (64, torch.float32)):
         check(sampler, rand(B, 151936, dtype, seed=B), some_ids(B, 151936, 1), 0.7, 20)

@@ -136,51 +136,71 @@ def test_embed_backward_workspace(lib):
     assert lib.zs_embed_backward_workspace(4, 8, None) == BAD
 
 
-# ---- top alternatives from one key per thread ----
+# ---- the bounds of the top alternatives, from one key per thread ----
 
-def _replay(x, k, head, N, nt, cl):
-    """What zs_logprobs_kernel does on a row whose first `head` elements precede the first
-    16-byte boundary, with N elements per vector, nt threads and cl CTAs: the candidates."""
+CODE_BITS = 12
+
+
+def _order(v):
+    """The kernels' 32-bit order of a float (NaN lowest)."""
+    if np.isnan(v):
+        return 0
+    u = int(np.float32(v + 0.0).view(np.uint32))
+    return u ^ 0xFFFFFFFF if u >> 31 else u | 0x80000000
+
+
+def _key(v, i):
+    return _order(v) << 32 | (~i & 0xFFFFFFFF)
+
+
+def _bounds(x, k, head, N, nt, cl):
+    """(rough, exact): the keys that zs_logprobs_kernel takes as lower bounds of the k best, on a
+    row whose first `head` elements precede the first 16-byte boundary, with N elements per
+    vector, nt threads and cl CTAs."""
     n = x.size
     head = min(head, n)
     nvec = (n - head) // N
     tail = n - head - nvec * N
-    groups = []  # (value, -position, span, element ids)
+    threads = []  # (rough key, exact key, up to its vector's last id)
     for r in range(cl):
         v0, v1 = nvec * r // cl, nvec * (r + 1) // cl
         for t in range(nt):
-            units = []
-            if r == 0 and t < head:
-                units.append((t, 1))
+            units = [(t, 1)] if r == 0 and t < head else []
             units += [(head + v * N, N) for v in range(v0 + t, v1, nt)]
             if r == cl - 1 and t < tail:
                 units.append((head + nvec * N + t, 1))
             if not units:
                 continue
-            best, pos, span = -np.inf, units[0][0], units[0][1]
+            best, (pos, span) = -np.inf, units[0]
             for p, s in units:
                 m = x[p:p + s].max()
                 if m > best:
                     best, pos, span = m, p, s
-            groups.append((best, -pos, span, [i for p, s in units for i in range(p, p + s)]))
-    groups.sort(key=lambda g: (g[0], g[1]), reverse=True)
-    sel = groups[:k]
-    if len(sel) < k:
-        return [i for g in sel for i in g[3]]
-    value, last = sel[-1][0], -sel[-1][1] + sel[-1][2] - 1
-    return [i for g in sel for i in g[3] if x[i] > value or (x[i] == value and i <= last)]
+            code = (1 << CODE_BITS) - 1 - (r * nt + t)
+            threads.append((_order(best) >> CODE_BITS << CODE_BITS | code, _key(best, pos + span - 1)))
+    threads.sort(reverse=True)
+    if len(threads) < k:
+        return 0, 0
+    sel = threads[:k]
+    return (sel[-1][0] >> CODE_BITS << CODE_BITS) << 32, min(e for _, e in sel)
 
 
 @pytest.mark.parametrize("kind", ["normal", "ties", "equal", "up", "down", "masked"])
 @pytest.mark.parametrize("n,head,N,nt,cl,k", [(997, 3, 4, 32, 1, 5), (997, 0, 8, 16, 4, 16),
                                               (50, 1, 8, 32, 2, 20), (33, 5, 8, 16, 1, 16),
-                                              (400, 2, 4, 64, 16, 33), (7, 0, 4, 8, 1, 5)])
-def test_the_best_groups_hold_the_top_alternatives(kind, n, head, N, nt, cl, k):
+                                              (400, 2, 4, 64, 8, 33), (7, 0, 4, 8, 1, 5)])
+def test_k_elements_reach_the_bounds(kind, n, head, N, nt, cl, k):
+    """At least k elements have a key at or above either bound, so the k best do; and
+    ties leave few above the exact one."""
     rng = np.random.default_rng(n + k)
     for _ in range(5):
         x = {"normal": rng.normal(size=n), "ties": np.round(rng.normal(size=n) * 2),
              "equal": np.zeros(n), "up": np.arange(n) * 1.0, "down": -np.arange(n) * 1.0,
              "masked": np.where(rng.random(n) < 0.97, -np.inf, rng.normal(size=n))}[kind]
-        want = sorted(range(n), key=lambda i: (-x[i], i))[:k]
-        cand = _replay(x, k, head, N, nt, cl)
-        assert len(cand) >= k and set(want) <= set(cand)
+        x = x.astype(np.float32)
+        keys = [_key(v, i) for i, v in enumerate(x)]
+        rough, exact = _bounds(x, k, head, N, nt, cl)
+        assert sum(q >= rough for q in keys) >= k
+        assert sum(q >= exact for q in keys) >= k
+        if kind == "equal" and exact:
+            assert sum(q >= exact for q in keys) <= nt * cl * N + head

@@ -576,8 +576,9 @@ struct EwArgs {
     EbArgs b;            // pair and part unused
     const int32_t* ids;
     int32_t zero;        // 1: zero the rows of other ids
-    int32_t bulk;        // bulk stores: rows start and end at 16-byte boundaries
-    int32_t group;       // rows per bulk store (a power of two up to 32, 1 if not contiguous)
+    int32_t group;       // rows per bulk store (a power of two up to 32; 1: rows not contiguous)
+    int32_t whole;       // whole groups start and end at 16-byte boundaries
+    int32_t rows;        // so does every row
 };
 // ids, ballots of two tokens, zeros, bits
 __host__ __device__ constexpr size_t ew_smem_bytes(int V) {
@@ -612,30 +613,39 @@ __global__ void __launch_bounds__(kEwThreads) zs_embed_few_kernel(const EwArgs a
             if (ids[i] >= 0) atomicOr(&bits[ids[i] >> 5], 1u << (ids[i] & 31));
         __syncthreads();
         const int64_t row_bytes = (int64_t)a.b.E * sizeof(TT);
-        if (a.bulk) {
-            const int groups = (V + a.group - 1) / a.group;
-            const uint32_t gmask = a.group == 32 ? ~0u : (1u << a.group) - 1u;
-            // a thread takes a group of rows: one store where none of them occurs
-            // (neighbouring groups go to different CTAs, so that all of them store)
+        const int groups = (V + a.group - 1) / a.group;
+        const uint32_t gmask = a.group == 32 ? ~0u : (1u << a.group) - 1u;
+        auto bulk_zero = [&](int r, int64_t bytes) {
+            uint8_t* p = reinterpret_cast<uint8_t*>(table + (int64_t)r * a.b.table_ld);
+            for (int64_t o = 0; o < bytes; o += kEwZeroBytes)
+                bulk_store(p + o, zeros, (uint32_t)min((int64_t)kEwZeroBytes, bytes - o));
+        };
+        // A thread takes a group of rows: one store where none of them occurs.
+        // (Neighbouring groups go to different CTAs, so that all of them store.)
+        if (a.whole) {
             for (int g = tid * gridDim.x + blockIdx.x; g < groups; g += gridDim.x * kEwThreads) {
                 const int r0 = g * a.group, nr = min(a.group, V - r0);
                 const uint32_t here = (bits[r0 >> 5] >> (r0 & 31)) & gmask;
-                for (int r = 0; r < nr; ++r) {
-                    if ((here >> r) & 1u) continue;
-                    const int cnt = here == 0u ? nr : 1;
-                    uint8_t* p = reinterpret_cast<uint8_t*>(table + (int64_t)(r0 + r) * a.b.table_ld);
-                    const int64_t bytes = row_bytes * cnt;
-                    for (int64_t o = 0; o < bytes; o += kEwZeroBytes)
-                        bulk_store(p + o, zeros, (uint32_t)min((int64_t)kEwZeroBytes, bytes - o));
-                    r += cnt - 1;
+                if (here == 0u && (a.rows || nr == a.group)) {
+                    bulk_zero(r0, row_bytes * nr);
+                } else if (a.rows) {
+                    for (int r = 0; r < nr; ++r)
+                        if (!((here >> r) & 1u)) bulk_zero(r0 + r, row_bytes);
                 }
             }
             asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-        } else {
-            for (int r = blockIdx.x * (kEwThreads / 32) + warp; r < V; r += gridDim.x * (kEwThreads / 32)) {
-                if ((bits[r >> 5] >> (r & 31)) & 1u) continue;
-                TT* p = table + (int64_t)r * a.b.table_ld;
-                for (int c = lane; c < a.b.E; c += 32) lp_store(p + c, 0.0f);
+        }
+        // What bulk stores cannot: single rows at other boundaries, a warp per group.
+        if (!a.rows) {
+            for (int g = blockIdx.x * (kEwThreads / 32) + warp; g < groups; g += gridDim.x * (kEwThreads / 32)) {
+                const int r0 = g * a.group, nr = min(a.group, V - r0);
+                const uint32_t here = (bits[r0 >> 5] >> (r0 & 31)) & gmask;
+                if (a.whole && here == 0u && nr == a.group) continue;
+                for (int r = 0; r < nr; ++r) {
+                    if ((here >> r) & 1u) continue;
+                    TT* p = table + (int64_t)(r0 + r) * a.b.table_ld;
+                    for (int c = lane; c < a.b.E; c += 32) lp_store(p + c, 0.0f);
+                }
             }
         }
     }
@@ -698,7 +708,7 @@ __global__ void __launch_bounds__(kEwThreads) zs_embed_few_kernel(const EwArgs a
             if (live) eb_write<TT>(a.b, (uint32_t)id, col, acc);
         }
     }
-    if (a.zero && a.bulk) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+    if (a.zero && a.whole) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
 }
 
 }  // namespace zs

@@ -33,7 +33,6 @@ constexpr int kLpMaxIds = 256;   // ZS_LOGPROBS_MAX_IDS
 constexpr int kLpMaxCl = 8;      // CTAs per row at most (one portable cluster)
 constexpr int kLpCandCap = 1536; // candidates ranked at once
 constexpr int kLpUnroll = 4;     // vectors in flight per thread
-constexpr int kLpSegVecs = 32 * kLpUnroll;  // a segment: what a warp takes at a time, 2 KB
 constexpr int kLpMaxSegs = 1024; // segment maxima a CTA keeps (2 MB of logits)
 constexpr int kLpMaxHits = 512;
 constexpr float kLpFloor = -200.0f;
@@ -505,6 +504,17 @@ __device__ __forceinline__ void lp_merge_lists(LpTopSmem<NT>& tp, int nl, int k,
     }
 }
 
+// Segments of a slice of nv vectors, and the first vector of one in its slice (the others
+// follow NT vectors apart); segments that begin past the slice's end are empty.
+template <int NT>
+__device__ __forceinline__ int lp_segments(int nv) {
+    return (nv + NT * kLpUnroll - 1) / (NT * kLpUnroll) * (NT / 32);
+}
+template <int NT>
+__device__ __forceinline__ int lp_segment_start(int s) {
+    return s / (NT / 32) * (NT * kLpUnroll) + s % (NT / 32) * 32;
+}
+
 // The two halves of a cluster barrier (every thread of every CTA of the cluster).
 __device__ __forceinline__ void cluster_arrive() {
     asm volatile("barrier.cluster.arrive.release;" ::: "memory");
@@ -520,8 +530,9 @@ __device__ __forceinline__ uint4 lp_stream(const uint4* p) {
 }
 
 // One row per cluster of a.cl CTAs (one CTA when a.cl is 1).  The row is streamed
-// once with 16-byte loads: a warp takes a segment of kLpUnroll x 32 vectors (2 KB) at a
-// time and loads its next one before it works on this.  The CTAs'
+// once with 16-byte loads: a warp takes kLpUnroll times 32 vectors (a segment of 2 KB,
+// one 512-byte piece of each quarter of what the CTA takes at a time) and loads its next
+// segment before it works on this.  The CTAs'
 // statistics meet in the leader (rank 0) through distributed shared memory in rank
 // order, so no scratch, no global atomics and a fixed summation order.
 //
@@ -578,13 +589,13 @@ __global__ void __launch_bounds__(NT, 1024 / NT) zs_logprobs_kernel(const LpArgs
         if (TOP && edge > st2.m) lp_raise2(st2, edge, c);
     }
     __shared__ LpTopSmem<TOP ? NT : 32> tp;
-    const int first = v0 + warp * 32 * kUnroll + lane;
+    const int first = v0 + tid;
     if (TOP && pos < 0 && first < v1) pos = cut.head + first * N;
-    const bool keep_segs = TOP && (v1 - v0 + kLpSegVecs - 1) / kLpSegVecs <= kLpMaxSegs;
+    const bool keep_segs = TOP && lp_segments<NT>(v1 - v0) <= kLpMaxSegs;
     uint4 q[kUnroll];
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u)
-        q[u] = first + u * 32 < v1 ? lp_stream<TOP>(xv + first + u * 32) : lp_fill(T());
+        q[u] = first + u * NT < v1 ? lp_stream<TOP>(xv + first + u * NT) : lp_fill(T());
     if constexpr (!TOP) {
         float m = -INFINITY;
 #pragma unroll
@@ -601,7 +612,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) zs_logprobs_kernel(const LpArgs
         uint4 next[kUnroll];
 #pragma unroll
         for (int u = 0; u < kUnroll; ++u) {
-            const int j = i + NT * kUnroll + u * 32;
+            const int j = i + NT * (kUnroll + u);
             next[u] = j < v1 ? lp_stream<TOP>(xv + j) : lp_fill(T());
         }
         if (!TOP && !masked && st2.m != -INFINITY) {
@@ -623,13 +634,13 @@ __global__ void __launch_bounds__(NT, 1024 / NT) zs_logprobs_kernel(const LpArgs
             const float b = lp_vec_max(q[u], T());
             if (b > m) {
                 m = b;
-                if (TOP) pos = cut.head + (i + u * 32) * N;
+                if (TOP) pos = cut.head + (i + u * NT) * N;
             }
             if (TOP) seg = fmaxf(seg, b);
         }
         if (TOP && keep_segs) {
             seg = lp_warp_max(seg);
-            if (lane == 0) tp.seg_max[(i - v0) / kLpSegVecs] = seg;
+            if (lane == 0) tp.seg_max[(i - v0) / (NT * kUnroll) * (NT / 32) + warp] = seg;
         }
         if (m > st2.m) {
             lp_raise2(st2, m, c);
@@ -711,7 +722,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) zs_logprobs_kernel(const LpArgs
         auto find = [&](bool loaded) {
             const int r = cl > 1 ? warp : 0, parts = cl > 1 ? 1 : kWarps;
             const int b0 = (int)((int64_t)cut.nvec * r / cl), b1 = (int)((int64_t)cut.nvec * (r + 1) / cl);
-            const int nseg = r < cl ? (b1 - b0 + kLpSegVecs - 1) / kLpSegVecs : 0;
+            const int nseg = r < cl ? lp_segments<NT>(b1 - b0) : 0;
             const bool kept = nseg <= kLpMaxSegs;
             const float* seg = (cl > 1 && r < cl ? cluster.map_shared_rank(&tp, r) : &tp)->seg_max;
             for (int i0 = (cl > 1 ? 0 : warp * 32 * kSegAhead); i0 < nseg; i0 += parts * 32 * kSegAhead) {
@@ -725,8 +736,8 @@ __global__ void __launch_bounds__(NT, 1024 / NT) zs_logprobs_kernel(const LpArgs
 #pragma unroll
                 for (int u = 0; u < kSegAhead; ++u) {
                     const int i = i0 + lane + u * 32;
-                    const int v = b0 + i * kLpSegVecs;  // the segment's first vector
-                    if (i < nseg && (!kept || make_key(ahead[u], cut.head + v * N) >= floor_key)) {
+                    const int v = b0 + lp_segment_start<NT>(i);  // the segment's first vector
+                    if (i < nseg && v < b1 && (!kept || make_key(ahead[u], cut.head + v * N) >= floor_key)) {
                         const int at = atomicAdd(&tp.nhits, 1);
                         if (at < kLpMaxHits) tp.hits[at] = v;
                     }
@@ -753,9 +764,9 @@ __global__ void __launch_bounds__(NT, 1024 / NT) zs_logprobs_kernel(const LpArgs
                 uint4 hq[kUnroll];
 #pragma unroll
                 for (int u = 0; u < kUnroll; ++u)
-                    if (seg0 + lane + u * 32 < end) hq[u] = xv[seg0 + lane + u * 32];
+                    if (seg0 + lane + u * NT < end) hq[u] = xv[seg0 + lane + u * NT];
 #pragma unroll 1
-                for (int v = seg0 + lane; v < min(end, seg0 + kLpSegVecs); v += 32) {
+                for (int v = seg0 + lane; v < min(end, seg0 + kUnroll * NT); v += NT) {
                     // a loop, not kUnroll copies of code that runs once
                     if (lp_vec_max(hq[0], T()) >= low_value || low_value != low_value) {
                         float e[N];

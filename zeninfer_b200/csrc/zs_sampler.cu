@@ -374,7 +374,7 @@ struct zs_context {
     int32_t lm_tiles = ZS_LMHEAD_TILES_AUTO;  // zs_set_lmhead_tiles
     int lm_pairs = 0;                         // resident CTA pairs of zs_lmhead_kernel<2>
     int32_t spec_mode = ZS_SPECULATION_ON;    // zs_set_speculation
-    int es_clusters = 2;                      // zs_embed_sort_kernel clusters of 4 resident at once
+    int es_clusters[2] = {2, 2};              // zs_embed_sort_kernel clusters of 4, 8 resident at once
     int small_clusters = 0;                   // zs_small_kernel clusters resident at once (0: none)
     int32_t small_max_rows = 8;               // zs_set_small_batch
     std::vector<TimedLaunch> timed;      // recorded since the last zs_get_timing
@@ -992,7 +992,7 @@ zs_status launch_embed_sort(zs_context* h, zs::EsArgs& e, cudaStream_t st) {
     e.sort_ctas = cl;
     const int ctas = e.zrows == 0 ? cl
                      : cl == 1    ? h->num_sms
-                                  : cl * (cl == 4 ? h->es_clusters : h->es_clusters / 2);
+                                  : cl * h->es_clusters[cl == 4 ? 0 : 1];
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = (unsigned)cl;
@@ -1022,10 +1022,12 @@ zs_status launch_embed_few(zs_context* h, const zs::EbArgs& b, const int32_t* id
     a.ids = ids;
     a.zero = !b.accumulate;
     const int64_t row = (int64_t)b.E * sizeof(TT);
-    a.bulk = !misaligned(b.table, 16) && row % 16 == 0 && b.table_ld * (int64_t)sizeof(TT) % 16 == 0;
+    const bool contiguous = b.table_ld == b.E, aligned = !misaligned(b.table, 16);
+    a.rows = aligned && row % 16 == 0 && b.table_ld * (int64_t)sizeof(TT) % 16 == 0;
     a.group = 1;
-    if (b.table_ld == b.E)
-        while (a.group < 32 && 2 * a.group * row <= (int64_t)zs::kEwZeroBytes) a.group *= 2;
+    if (contiguous)  // groups of 16 KB at most, but of 8 rows at least, which always fit 16 bytes
+        while (a.group < 32 && (a.group < 8 || 2 * a.group * row <= (int64_t)zs::kEwZeroBytes)) a.group *= 2;
+    a.whole = a.rows || (contiguous && aligned);
     LaunchScope scope(h, -1, st);
     const int ctas = a.zero ? 2 * h->num_sms : std::min(b.n, 2 * h->num_sms);
     k<<<ctas, zs::kEwThreads, smem, st>>>(a);
@@ -1129,15 +1131,15 @@ zs_status zs_create(int device, zs_handle* out) {
     if ((e = cudaFuncSetAttribute(zs::zs_embed_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                   (int)sizeof(zs::EsSmem))) != cudaSuccess)
         return cleanup(cuda_fail(e, "cudaFuncSetAttribute zs_embed_sort_kernel"));
-    {
+    for (int i = 0; i < 2; ++i) {  // clusters of four and of eight resident at once
         cudaLaunchAttribute attr[1];
         attr[0].id = cudaLaunchAttributeClusterDimension;
-        attr[0].val.clusterDim.x = 4;
+        attr[0].val.clusterDim.x = i == 0 ? 4 : 8;
         attr[0].val.clusterDim.y = 1;
         attr[0].val.clusterDim.z = 1;
         cudaLaunchConfig_t cfg;
         std::memset(&cfg, 0, sizeof(cfg));
-        cfg.gridDim = dim3(4);
+        cfg.gridDim = dim3(attr[0].val.clusterDim.x);
         cfg.blockDim = dim3(zs::kEsThreads);
         cfg.dynamicSmemBytes = sizeof(zs::EsSmem);
         cfg.attrs = attr;
@@ -1145,7 +1147,7 @@ zs_status zs_create(int device, zs_handle* out) {
         int nc = 0;
         if ((e = cudaOccupancyMaxActiveClusters(&nc, zs::zs_embed_sort_kernel, &cfg)) != cudaSuccess)
             return cleanup(cuda_fail(e, "occupancy of zs_embed_sort_kernel"));
-        h->es_clusters = std::max(4, nc);
+        h->es_clusters[i] = std::max(2, nc);
     }
     // CTA pairs of the lm_head kernel that can be resident at once (0: none; the
     // one-CTA tiles are used then).
