@@ -504,15 +504,19 @@ __device__ __forceinline__ void lp_merge_lists(LpTopSmem<NT>& tp, int nl, int k,
     }
 }
 
-// Segments of a slice of nv vectors, and the first vector of one in its slice (the others
-// follow NT vectors apart); segments that begin past the slice's end are empty.
+// Segments of a slice of nv vectors, how far apart their pieces lie, and the first vector
+// of one in its slice; segments that begin past the slice's end are empty.
 template <int NT>
 __device__ __forceinline__ int lp_segments(int nv) {
     return (nv + NT * kLpUnroll - 1) / (NT * kLpUnroll) * (NT / 32);
 }
-template <int NT>
+template <int NT, bool TOP>
+__host__ __device__ constexpr int lp_piece_step() {
+    return TOP ? NT : 32;
+}
+template <int NT, bool TOP>
 __device__ __forceinline__ int lp_segment_start(int s) {
-    return s / (NT / 32) * (NT * kLpUnroll) + s % (NT / 32) * 32;
+    return s / (NT / 32) * (NT * kLpUnroll) + s % (NT / 32) * (TOP ? 32 : 32 * kLpUnroll);
 }
 
 // The two halves of a cluster barrier (every thread of every CTA of the cluster).
@@ -530,9 +534,10 @@ __device__ __forceinline__ uint4 lp_stream(const uint4* p) {
 }
 
 // One row per cluster of a.cl CTAs (one CTA when a.cl is 1).  The row is streamed
-// once with 16-byte loads: a warp takes kLpUnroll times 32 vectors (a segment of 2 KB,
-// one 512-byte piece of each quarter of what the CTA takes at a time) and loads its next
-// segment before it works on this.  The CTAs'
+// once with 16-byte loads: a warp takes a segment of kLpUnroll pieces of 32 vectors (2 KB in
+// a row; in short slices with alternatives the pieces lie NT vectors apart, so that as
+// many threads as possible hold a vector) and loads its next segment before it works on
+// this.  The CTAs'
 // statistics meet in the leader (rank 0) through distributed shared memory in rank
 // order, so no scratch, no global atomics and a fixed summation order.
 //
@@ -589,13 +594,14 @@ __global__ void __launch_bounds__(NT, 1024 / NT) zs_logprobs_kernel(const LpArgs
         if (TOP && edge > st2.m) lp_raise2(st2, edge, c);
     }
     __shared__ LpTopSmem<TOP ? NT : 32> tp;
-    const int first = v0 + tid;
+    constexpr int step = lp_piece_step<NT, TOP>();
+    const int first = v0 + lp_segment_start<NT, TOP>(warp) + lane;
     if (TOP && pos < 0 && first < v1) pos = cut.head + first * N;
     const bool keep_segs = TOP && lp_segments<NT>(v1 - v0) <= kLpMaxSegs;
     uint4 q[kUnroll];
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u)
-        q[u] = first + u * NT < v1 ? lp_stream<TOP>(xv + first + u * NT) : lp_fill(T());
+        q[u] = first + u * step < v1 ? lp_stream<TOP>(xv + first + u * step) : lp_fill(T());
     if constexpr (!TOP) {
         float m = -INFINITY;
 #pragma unroll
@@ -612,7 +618,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) zs_logprobs_kernel(const LpArgs
         uint4 next[kUnroll];
 #pragma unroll
         for (int u = 0; u < kUnroll; ++u) {
-            const int j = i + NT * (kUnroll + u);
+            const int j = i + NT * kUnroll + u * step;
             next[u] = j < v1 ? lp_stream<TOP>(xv + j) : lp_fill(T());
         }
         if (!TOP && !masked && st2.m != -INFINITY) {
@@ -634,7 +640,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) zs_logprobs_kernel(const LpArgs
             const float b = lp_vec_max(q[u], T());
             if (b > m) {
                 m = b;
-                if (TOP) pos = cut.head + (i + u * NT) * N;
+                if (TOP) pos = cut.head + (i + u * step) * N;
             }
             if (TOP) seg = fmaxf(seg, b);
         }
@@ -736,7 +742,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) zs_logprobs_kernel(const LpArgs
 #pragma unroll
                 for (int u = 0; u < kSegAhead; ++u) {
                     const int i = i0 + lane + u * 32;
-                    const int v = b0 + lp_segment_start<NT>(i);  // the segment's first vector
+                    const int v = b0 + lp_segment_start<NT, TOP>(i);  // its first vector
                     if (i < nseg && v < b1 && (!kept || make_key(ahead[u], cut.head + v * N) >= floor_key)) {
                         const int at = atomicAdd(&tp.nhits, 1);
                         if (at < kLpMaxHits) tp.hits[at] = v;
@@ -764,9 +770,9 @@ __global__ void __launch_bounds__(NT, 1024 / NT) zs_logprobs_kernel(const LpArgs
                 uint4 hq[kUnroll];
 #pragma unroll
                 for (int u = 0; u < kUnroll; ++u)
-                    if (seg0 + lane + u * NT < end) hq[u] = xv[seg0 + lane + u * NT];
+                    if (seg0 + lane + u * step < end) hq[u] = xv[seg0 + lane + u * step];
 #pragma unroll 1
-                for (int v = seg0 + lane; v < min(end, seg0 + kUnroll * NT); v += NT) {
+                for (int v = seg0 + lane; v < min(end, seg0 + kUnroll * step); v += step) {
                     // a loop, not kUnroll copies of code that runs once
                     if (lp_vec_max(hq[0], T()) >= low_value || low_value != low_value) {
                         float e[N];
