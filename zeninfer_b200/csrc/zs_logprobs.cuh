@@ -312,7 +312,9 @@ __device__ __forceinline__ void lp_add2(LpStat2& a, float lo, float hi, uint64_t
 // off by up to t 2^-23): it starts as the largest of the CTA's first 8 or 16 KB segments
 // and is raised when a thread's sum passes 2^24, which saves the maximum of nearly all
 // vectors; and t is clamped only once a product e t came out NaN, that is after the
-// first -inf.  4096 bf16 rows of 151,936: 201 -> 192 us.
+// first -inf.  4096 bf16 rows of 151,936: 201 -> 187 us (6.6 TB/s).  (A quarter of the
+// exponentials as polynomials on the FMA pipes was slower, 200 us: the pass is bound by
+// HBM and issue slots before the special-function unit.)
 constexpr float kLpLazyLimit = 16777216.0f;
 template <int U>
 __device__ __forceinline__ void lp_add_plain(LpStat2& a, const uint4 (&q)[U], float c, float) {
