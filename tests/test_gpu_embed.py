@@ -195,6 +195,41 @@ def test_embed_backward_strides_streams_and_graphs(sampler):
             assert torch.equal(got, ref)
 
 
+def test_offsets_past_32_bits(sampler):
+    V, E = 2_800_000, 800  # 2.24 G elements
+    table = torch.zeros(V, E, dtype=torch.float16, device="cuda")
+    ids = torch.tensor([V - 1, 0, V - 2, 5, V - 1], dtype=torch.int32, device="cuda")
+    grad = torch.randint(-4, 5, (5, E), device="cuda").to(torch.float16)
+    for n in (5, 2000):  # above 1024 tokens, and above 2^19 ids, the sorted way
+        i2, g2 = ids.repeat(n // 5), grad.repeat(n // 5, 1)
+        table.fill_(1.0)
+        sampler.embed_backward(g2, i2, V, out=table)
+        assert torch.equal(table[V - 1], (grad[0] + grad[4]) * (n // 5))
+        assert torch.equal(table[V - 2], grad[2] * (n // 5)) and torch.equal(table[5], grad[3] * (n // 5))
+        assert not table[6:V - 2].any() and not table[1:5].any()
+    assert torch.equal(sampler.embed(table, ids), table[ids.long()])
+    wide = torch.as_strided(table, (2, E), (V * E - E, 1))
+    assert torch.equal(sampler.embed(table[:3], torch.zeros(2, dtype=torch.int32, device="cuda"), 1.0,
+                                     out=wide), table[[0, V - 1]])
+
+
+def test_embed_backward_on_two_streams_at_once(sampler):
+    n, V, E = 9000, 4000, 64
+    g = torch.Generator(device="cuda").manual_seed(8)
+    grads = [torch.randn(n, E, generator=g, device="cuda") for _ in range(2)]
+    ids = [ids_of(n, V, seed=40 + i) for i in range(2)]
+    want = [sampler.embed_backward(grads[i], ids[i], V) for i in range(2)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = []
+    for _ in range(8):
+        for i, st in enumerate(streams):
+            got.append((i, sampler.embed_backward(grads[i], ids[i], V, stream=st)))
+    torch.cuda.synchronize()
+    for i, t in got:
+        assert torch.equal(t, want[i])
+
+
 def test_embed_backward_against_differences(sampler):
     """The loss sum(embed(table) * grad) is linear in the table: its difference quotient is
     the gradient (64-bit sums; f32 roundings of a few terms of order 1)."""

@@ -170,6 +170,38 @@ def test_sorted_rows(sampler, B):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("B", [1, 9, 200])
+@pytest.mark.parametrize("top", [0, 2])
+def test_rows_that_outgrow_their_beginning(sampler, dtype, B, top):
+    """Values that rise by far more than the exponential's range, a single peak at the
+    end, a fall from a first peak, and a first part without any token."""
+    V = 40013
+    x = rand(B, V, dtype, seed=21)
+    ramp = torch.linspace(-300, 300, V, device="cuda")
+    rows = [x + ramp, x - ramp, x.clone(), x.clone(), x.clone()]
+    rows[2][:, V - 1] = 60000.0
+    rows[3][:, 0] = 500.0
+    rows[4][:, :V - 900] = -math.inf
+    for y in rows:
+        check(sampler, y.to(dtype), some_ids(B, V, 1), 1.0, top)
+        check(sampler, y.to(dtype), some_ids(B, V, 1), 0.1, top)
+        check(sampler, y.to(dtype), some_ids(B, V, 1), 30.0, top)
+
+
+def test_offsets_past_32_bits(sampler):
+    V, ld = 1500, (1 << 31) + 8
+    buf = torch.empty(ld + V, dtype=torch.float16, device="cuda")
+    x = torch.as_strided(buf, (2, V), (ld, 1), 0)
+    x.copy_(rand(2, V, torch.float16, seed=22))
+    ids = some_ids(2, V, 1)
+    r = check(sampler, x, ids, 1.0, 5)
+    gl = torch.ones(2, 1, device="cuda")
+    want = sampler.logprobs_backward(x.contiguous(), r.rows, ids, gl)
+    sampler.logprobs_backward(x, r.rows, ids, gl, out=x)
+    assert torch.equal(x, want)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("B", [4, 150])
 def test_masked_rows(sampler, dtype, B):
     V = 12001
@@ -384,6 +416,34 @@ def test_streams_graphs_and_repeats(sampler):
         assert torch.equal(g, ref_g)
 
 
+def test_two_streams_at_once(sampler):
+    """Calls that overlap on the GPU share nothing."""
+    B, V = 300, 30011
+    xs = [rand(B, V, torch.float32, seed=30 + i) for i in range(2)]
+    ids = some_ids(B, V, 1)
+    gl = torch.ones(B, 1, device="cuda")
+    hidden, norm, w = lm_inputs(64, 5000, 256, seed=9)
+    want = [sampler.logprobs(x, ids, top=20) for x in xs]
+    want_g = [sampler.logprobs_backward(x, r.rows, ids, gl) for x, r in zip(xs, want)]
+    want_l = [sampler.lmhead_logprobs(hidden * (i + 1), norm, w, temp=1.0 + i) for i in range(2)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    hs = [hidden * (i + 1) for i in range(2)]
+    torch.cuda.synchronize()
+    for _ in range(6):
+        for i, st in enumerate(streams):
+            r = sampler.logprobs(xs[i], ids, top=20, stream=st)
+            g = sampler.logprobs_backward(xs[i], r.rows, ids, gl, stream=st)
+            got[i].append((r, g, sampler.lmhead_logprobs(hs[i], norm, w, temp=1.0 + i, stream=st)))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for r, g, lm in got[i]:
+            assert torch.equal(r.logp, want[i].logp) and torch.equal(r.top_ids, want[i].top_ids)
+            assert torch.equal(g, want_g[i])
+            assert torch.equal(lm.lse, want_l[i].lse) and torch.equal(lm.entropy, want_l[i].entropy)
+
+
 def test_empty_and_no_ids(sampler):
     r = sampler.logprobs(torch.empty(0, 100, device="cuda"), top=3)
     assert r.entropy.shape == (0,) and r.top_ids.shape == (0, 3) and r.logp is None
@@ -439,7 +499,9 @@ def lm_exact(hidden, norm, w, eps=1e-6):
 
 
 @pytest.mark.parametrize("B,V,E,m", [(1, 1000, 64, 1), (3, 129, 72, 2), (16, 5003, 896, 1),
-                                     (130, 4099, 256, 3), (513, 3001, 128, 1), (700, 20000, 64, 1)])
+                                     (8, 1, 64, 1), (127, 300, 80, 1),
+                                     (130, 4099, 256, 3), (513, 3001, 128, 1), (700, 20000, 64, 1),
+                                     (4500, 700, 64, 1), (9000, 300, 64, 2), (6, 90, 12288, 1)])
 def test_lmhead_logprobs(sampler, B, V, E, m):
     """The logits are f32 accumulations of exact products, 16 at a time: each of the E / 16
     steps (and one within) is off by at most a step, 2^-23, of the sum of magnitudes."""
@@ -474,10 +536,29 @@ def test_lmhead_logprobs_agrees_with_its_parts(sampler):
         assert float((getattr(a, name) - getattr(b, name)).abs().max()) <= tol
 
 
-@pytest.mark.parametrize("mode", ["single", "pair"])
-def test_lmhead_logprobs_tiles(sampler, mode):
-    hidden, norm, w = lm_inputs(300, 2500, 192, seed=4)
-    ids = some_ids(300, 2500, 1)
+def test_lmhead_logprobs_of_large_logits(sampler):
+    """Logits of hundreds: the base of the sums has to move, by more than the exponential's
+    range within a tile.  Tolerances as above (they grow with the logits)."""
+    B, V, E = 40, 3000, 128
+    hidden, norm, w = lm_inputs(B, V, E, seed=6)
+    w = (w.float() * 60).to(torch.bfloat16)
+    w[V - 1] *= 8
+    ids = some_ids(B, V, 1)
+    x, size = lm_exact(hidden, norm, w)
+    lse, h, logp, t_sum, t_lse, t_h = exact(x, torch.ones(B, dtype=torch.float64, device="cuda"))
+    r = sampler.lmhead_logprobs(hidden, norm, w, ids)
+    off = (E / 16 + 2) * 2 ** -23 * size
+    e1 = (logp.exp() * (logp - logp.max(1, keepdim=True).values).abs()).sum(1)
+    close(r.lse, lse, t_lse + off, "lse")
+    close(r.entropy, h, t_h + 2 * off * (1 + e1), "entropy")
+    want = torch.where(ids >= 0, torch.gather(logp, 1, ids.clamp(min=0).long()), 0.0)
+    close(r.logp, want, (t_sum + 2 * off)[:, None] + want.abs() * U, "logp")
+
+
+@pytest.mark.parametrize("mode,B", [("single", 300), ("pair", 300), ("single", 2300), ("pair", 2300)])
+def test_lmhead_logprobs_tiles(sampler, mode, B):
+    hidden, norm, w = lm_inputs(B, 2500, 192, seed=4)
+    ids = some_ids(B, 2500, 1)
     ref = sampler.lmhead_logprobs(hidden, norm, w, ids)
     sampler.set_lmhead_tiles(mode)
     try:

@@ -94,7 +94,7 @@ def _embed(lib, h, table=P, td=BF16, tld=64, V=100, E=64, ids=P, n=3, out=P, od=
     dict(table=None), dict(table=P + 1), dict(td=3), dict(od=-1), dict(tld=63), dict(old=63),
     dict(V=0), dict(E=0), dict(E=(1 << 20) + 1, tld=1 << 21, old=1 << 21), dict(ids=None),
     dict(ids=P + 1), dict(n=-1), dict(n=(1 << 30) + 1), dict(out=None), dict(out=P + 2),
-    dict(tld=(1 << 30) + 1), dict(old=(1 << 30) + 1),
+    dict(tld=(1 << 40) + 1), dict(old=(1 << 40) + 1),
 ])
 def test_embed_refuses(lib, handle, change):
     assert _embed(lib, handle, **change) == BAD
@@ -108,7 +108,7 @@ def _embed_backward(lib, h, g=P, gd=BF16, gld=64, ids=P, n=3, V=100, E=64, t=P, 
 @pytest.mark.parametrize("change", [
     dict(g=None), dict(g=P + 1), dict(gd=3), dict(td=3), dict(gld=63), dict(tld=63), dict(V=0),
     dict(E=0), dict(ids=None), dict(ids=P + 2), dict(n=-1), dict(n=(1 << 30) + 1), dict(t=None),
-    dict(t=P + 2), dict(ws=None), dict(ws=P + 128), dict(wsb=100), dict(tld=(1 << 30) + 1),
+    dict(t=P + 2), dict(ws=None), dict(ws=P + 128), dict(wsb=100), dict(tld=(1 << 40) + 1),
 ])
 def test_embed_backward_refuses(lib, handle, change):
     assert _embed_backward(lib, handle, **change) == BAD

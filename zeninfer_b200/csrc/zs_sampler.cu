@@ -2134,7 +2134,7 @@ zs_status zs_embed(zs_handle h, const void* table, int32_t table_dtype, int64_t 
         return fail(ZS_ERR_INVALID_ARGUMENT, "table, ids or out not aligned to its type");
     if (table_ld < n_embd || out_ld < n_embd)
         return fail(ZS_ERR_INVALID_ARGUMENT, "table_ld or out_ld < n_embd");
-    if (table_ld > (int64_t)1 << 30 || out_ld > (int64_t)1 << 30)
+    if (table_ld > (int64_t)1 << 40 || out_ld > (int64_t)1 << 40)
         return fail(ZS_ERR_INVALID_ARGUMENT, "table_ld or out_ld too large");
     DeviceGuard g(h->device);
     if (!g.ok) return fail(ZS_ERR_CUDA, "cudaSetDevice failed");
@@ -2182,13 +2182,13 @@ zs_status zs_embed_backward(zs_handle h, const void* grad_out, int32_t grad_dtyp
         return fail(ZS_ERR_INVALID_ARGUMENT, "n_embd must be 1 to ZS_EMBED_MAX_EMBD");
     if (!grad_table || misaligned(grad_table, ts))
         return fail(ZS_ERR_INVALID_ARGUMENT, "grad_table is null or not aligned to its type");
-    if (table_ld < n_embd || table_ld > (int64_t)1 << 30)
+    if (table_ld < n_embd || table_ld > (int64_t)1 << 40)
         return fail(ZS_ERR_INVALID_ARGUMENT, "table_ld < n_embd or too large");
     if (n_tokens > 0) {
         if (!grad_out || !ids) return fail(ZS_ERR_INVALID_ARGUMENT, "grad_out or ids is null");
         if (misaligned(grad_out, gs) || misaligned(ids, 4))
             return fail(ZS_ERR_INVALID_ARGUMENT, "grad_out or ids not aligned to its type");
-        if (grad_ld < n_embd || grad_ld > (int64_t)1 << 30)
+        if (grad_ld < n_embd || grad_ld > (int64_t)1 << 40)
             return fail(ZS_ERR_INVALID_ARGUMENT, "grad_ld < n_embd or too large");
         if (!workspace || misaligned(workspace, 256) ||
             workspace_bytes < embed_ws(n_tokens, n_embd).total)
