@@ -562,14 +562,20 @@ __global__ void __launch_bounds__(kEbThreads * kEjGroups) zs_embed_join_kernel(c
 }
 
 // ---- gradient: few tokens, in one launch ----
-// Up to kEwMaxTokens tokens need no sort: every CTA holds all ids in shared memory, and
-// the CTA that takes token i finds the positions of its id by comparing them all (a
-// ballot per 32), sums those rows in order if i is the first of them, and writes the
-// table row.  The rows of ids that do not occur (a bit per row) are zeroed by bulk
-// stores issued before the sums, so the two overlap.
+// Up to kEwMaxTokens tokens need no sort: every CTA holds all ids in shared memory.  A
+// warp takes a token and 32 G of the columns, finds the positions of the token's id by
+// comparing them all (a ballot per 32), and, if the token is the first of them, sums those
+// rows in order and writes its part of the table row.  A run of more than kEwLong rows (a
+// padding id) is left to all warps of the CTA, which share its positions and add their
+// sums in order.  The rows of ids that do not occur (a bit per row) are zeroed by bulk
+// stores issued before the sums, so the two overlap.  Against the sorted way, 1000 bf16
+// rows of 896 added to a 32,000-row f32 table: 11.9 against 23.0 us with a natural
+// frequency law, 23.7 against 17.5 when all are one id; at 2048 tokens both take 23.
 constexpr int kEwMaxTokens = 1024;
 constexpr int kEwMaxVocab = 1 << 19;  // the bits take 64 KB at most
 constexpr int kEwThreads = 256;
+constexpr int kEwWarps = kEwThreads / 32;
+constexpr int kEwLong = 16;
 constexpr uint32_t kEwZeroBytes = 16u << 10;
 
 struct EwArgs {
@@ -580,9 +586,9 @@ struct EwArgs {
     int32_t whole;       // whole groups start and end at 16-byte boundaries
     int32_t rows;        // so does every row
 };
-// ids, ballots of two tokens, zeros, bits
+// zeros, ids, the warps' sums of a long run, bits
 __host__ __device__ constexpr size_t ew_smem_bytes(int V) {
-    return kEwMaxTokens * 4 + 2 * (kEwMaxTokens / 32) * 4 + kEwZeroBytes + ((size_t)V + 31) / 32 * 4;
+    return kEwZeroBytes + kEwMaxTokens * 4 + kEwWarps * 32 * 8 * 4 + ((size_t)V + 31) / 32 * 4;
 }
 
 template <typename TG, typename TT, bool VEC>
@@ -592,8 +598,9 @@ __global__ void __launch_bounds__(kEwThreads) zs_embed_few_kernel(const EwArgs a
     extern __shared__ __align__(128) uint8_t ew_raw[];
     uint4* zeros = reinterpret_cast<uint4*>(ew_raw);
     int32_t* ids = reinterpret_cast<int32_t*>(ew_raw + kEwZeroBytes);
-    uint32_t* ballots = reinterpret_cast<uint32_t*>(ids + kEwMaxTokens);  // [2][kEwMaxTokens / 32]
-    uint32_t* bits = ballots + 2 * (kEwMaxTokens / 32);
+    float* part = reinterpret_cast<float*>(ids + kEwMaxTokens);  // [kEwWarps][32 * 8]
+    uint32_t* bits = reinterpret_cast<uint32_t*>(part + kEwWarps * 32 * 8);
+    __shared__ int64_t long_task[kEwWarps];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int n = a.b.n, V = a.b.V, words = (V + 31) / 32;
     for (int i = tid; i < kEwMaxTokens; i += kEwThreads) {
@@ -650,62 +657,94 @@ __global__ void __launch_bounds__(kEwThreads) zs_embed_few_kernel(const EwArgs a
         }
     }
     const int blocks = (n + 31) / 32;
-    int turn = 0;
-    for (int i = blockIdx.x; i < n; i += gridDim.x) {
-        const int32_t id = ids[i];
-        if (id < 0) continue;  // the same for the whole CTA
-        uint32_t* mine = ballots + turn * (kEwMaxTokens / 32);
-        turn ^= 1;
-        for (int b = warp; b < blocks; b += kEwThreads / 32) {
-            const uint32_t m = __ballot_sync(kFull, ids[b * 32 + lane] == id);
-            if (lane == 0) mine[b] = m;
-        }
-        // One barrier per turn: these words were read two turns ago, before the last
-        // turn's barrier.
-        __syncthreads();
-        // lane b holds the ballot of positions 32 b .. 32 b + 31
-        const uint32_t word = lane < blocks ? mine[lane] : 0u;
-        const uint32_t before = lane < i >> 5 ? ~0u : lane == i >> 5 ? (1u << (i & 31)) - 1u : 0u;
-        if (__any_sync(kFull, (word & before) != 0u)) continue;  // not its first position
-        const uint32_t some = __ballot_sync(kFull, word != 0u);
-        // every lane of a warp stays: the ballots are handed round by shuffles
-        for (int c0 = warp * 32 * G; c0 < a.b.E; c0 += kEwThreads * G) {
-            const int col = c0 + lane * G;
-            const bool live = col < a.b.E;
-            const TG* grad = reinterpret_cast<const TG*>(a.b.grad) + (live ? col : 0);
-            float acc[G];
+    static_assert(kEwMaxTokens % (32 * 8) == 0, "whole groups of compared blocks");
+    const int tiles = (a.b.E + 32 * G - 1) / (32 * G);
+    const int64_t tasks = (int64_t)n * tiles;
+    float acc[G];
+    // Adds the rows at up to `left` positions of `id` in blocks b, b + step, .. of 32, in
+    // order, for this lane's columns (col on; none if not live).  The whole warp takes part.
+    auto add_rows = [&](int32_t id, int b, int step, int left, int col, bool live) {
+        const TG* grad = reinterpret_cast<const TG*>(a.b.grad) + (live ? col : 0);
+        constexpr int kAhead = 8;
+        uint32_t m = 0u;
+        int at = 0;
 #pragma unroll
-            for (int j = 0; j < G; ++j) acc[j] = 0.0f;
-            constexpr int kAhead = 8;
-            uint32_t left = some, m = 0u;
-            int b = 0;
-            while ((left | m) != 0u) {
-                Raw q[kAhead];
-                int got = 0;
+        for (int j = 0; j < G; ++j) acc[j] = 0.0f;
+        for (bool more = true; more;) {
+            Raw q[kAhead];
+            int got = 0;
 #pragma unroll
-                for (int u = 0; u < kAhead; ++u) {
-                    if (m == 0u && left != 0u) {
-                        b = __ffs(left) - 1;
-                        left &= left - 1u;
-                        m = __shfl_sync(kFull, word, b);
-                    }
-                    if (m != 0u) {
-                        if (live) q[u] = eb_load<G>(grad + (int64_t)(b * 32 + __ffs(m) - 1) * a.b.grad_ld);
-                        m &= m - 1u;
-                        got = u + 1;
-                    }
+            for (int u = 0; u < kAhead; ++u) {
+                while (m == 0u && b < blocks && left > 0) {
+                    m = __ballot_sync(kFull, ids[b * 32 + lane] == id);
+                    at = b * 32;
+                    b += step;
+                    left -= __popc(m);
                 }
-#pragma unroll
-                for (int u = 0; u < kAhead; ++u) {
-                    if (u < got && live) {
-                        float v[G];
-                        eb_unpack(q[u], v, TG());
-#pragma unroll
-                        for (int j = 0; j < G; ++j) acc[j] += v[j];
-                    }
+                if (m != 0u) {
+                    if (live) q[u] = eb_load<G>(grad + (int64_t)(at + __ffs(m) - 1) * a.b.grad_ld);
+                    m &= m - 1u;
+                    got = u + 1;
                 }
             }
-            if (live) eb_write<TT>(a.b, (uint32_t)id, col, acc);
+            more = got == kAhead;
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u) {
+                if (u < got && live) {
+                    float v[G];
+                    eb_unpack(q[u], v, TG());
+#pragma unroll
+                    for (int j = 0; j < G; ++j) acc[j] += v[j];
+                }
+            }
+        }
+    };
+    // Neighbouring tasks (the columns of one token) go to different CTAs.
+    for (int64_t base = blockIdx.x; base < tasks; base += (int64_t)gridDim.x * kEwWarps) {
+        const int64_t task = base + (int64_t)warp * gridDim.x;
+        bool is_long = false;
+        if (task < tasks) {
+            const int i = (int)(task / tiles), t = (int)(task - (int64_t)i * tiles);
+            const int32_t id = ids[i];
+            int count = id >= 0 ? 0 : -1;  // -1: nothing to do
+            constexpr int kScan = 8;       // blocks compared side by side
+            for (int b0 = 0; b0 < blocks && count >= 0; b0 += kScan) {
+                uint32_t before = 0u;
+#pragma unroll
+                for (int u = 0; u < kScan; ++u) {
+                    const int b = b0 + u;  // (past the last token the ids are -1)
+                    const uint32_t m = __ballot_sync(kFull, ids[b * 32 + lane] == id);
+                    before |= b < i >> 5 ? m : b == i >> 5 ? m & ((1u << (i & 31)) - 1u) : 0u;
+                    count += __popc(m);
+                }
+                if (before != 0u) count = -1;
+            }
+            is_long = count > kEwLong;
+            if (count > 0 && !is_long) {
+                const int col = (t * 32 + lane) * G;
+                add_rows(id, i >> 5, 1, count, col, col < a.b.E);
+                if (col < a.b.E) eb_write<TT>(a.b, (uint32_t)id, col, acc);
+            }
+        }
+        if (lane == 0) long_task[warp] = is_long ? task : -1;
+        if (__syncthreads_or(is_long)) {
+            for (int w = 0; w < kEwWarps; ++w) {
+                const int64_t lt = long_task[w];
+                if (lt < 0) continue;  // the same for the whole CTA
+                const int i = (int)(lt / tiles), t = (int)(lt - (int64_t)i * tiles);
+                const int col = (t * 32 + lane) * G;
+                add_rows(ids[i], warp, kEwWarps, n, col, col < a.b.E);
+#pragma unroll
+                for (int j = 0; j < G; ++j) part[(warp * 32 + lane) * G + j] = acc[j];
+                __syncthreads();
+                if (warp == 0 && col < a.b.E) {
+                    for (int y = 1; y < kEwWarps; ++y)
+#pragma unroll
+                        for (int j = 0; j < G; ++j) acc[j] += part[(y * 32 + lane) * G + j];
+                    eb_write<TT>(a.b, (uint32_t)ids[i], col, acc);
+                }
+                __syncthreads();
+            }
         }
     }
     if (a.zero && a.whole) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");

@@ -1010,13 +1010,14 @@ zs_status launch_embed_sort(zs_context* h, zs::EsArgs& e, cudaStream_t st) {
     return ZS_OK;
 }
 
-// Few tokens: one launch, two CTAs per SM.
+// Few tokens: one launch, up to four CTAs per SM.
 template <typename TG, typename TT, bool VEC>
 zs_status launch_embed_few(zs_context* h, const zs::EbArgs& b, const int32_t* ids, cudaStream_t st) {
     auto k = zs::zs_embed_few_kernel<TG, TT, VEC>;
     const size_t smem = zs::ew_smem_bytes(b.V);
-    ZS_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 (int)zs::ew_smem_bytes(zs::kEwMaxVocab)));
+    if (smem > 40u << 10)  // (with the static part, 48 KB go without)
+        ZS_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                     (int)zs::ew_smem_bytes(zs::kEwMaxVocab)));
     zs::EwArgs a;
     a.b = b;
     a.ids = ids;
@@ -1029,8 +1030,11 @@ zs_status launch_embed_few(zs_context* h, const zs::EbArgs& b, const int32_t* id
         while (a.group < 32 && (a.group < 8 || 2 * a.group * row <= (int64_t)zs::kEwZeroBytes)) a.group *= 2;
     a.whole = a.rows || (contiguous && aligned);
     LaunchScope scope(h, -1, st);
-    const int ctas = a.zero ? 2 * h->num_sms : std::min(b.n, 2 * h->num_sms);
-    k<<<ctas, zs::kEwThreads, smem, st>>>(a);
+    constexpr int G = zs::EbGran<TG, TT, VEC>::G;
+    const int64_t tasks = (int64_t)b.n * ((b.E + 32 * G - 1) / (32 * G));
+    const int64_t most = 4 * h->num_sms;
+    const int64_t ctas = a.zero ? most : std::min<int64_t>(most, tasks);
+    k<<<(unsigned)ctas, zs::kEwThreads, smem, st>>>(a);
     ZS_CUDA(cudaGetLastError());
     return ZS_OK;
 }
