@@ -5,8 +5,9 @@
 //   grad_table[v] = scale * sum_{i: ids[i] == v} grad_out[i]
 //
 // The gradient is taken by sorted tokens: (id, position) pairs are sorted (stable), and
-// each id's rows are summed in f32 in the order of their positions, chunk by chunk, so
-// the result does not depend on timing and each table row is rounded once.
+// each id's rows are summed in f32 in the order of their positions, chunk by chunk; up to
+// 1024 tokens their positions are found by comparing all ids instead.  Either way the
+// result does not depend on timing and each table row is rounded once.
 #pragma once
 
 #include <cooperative_groups.h>

@@ -45,7 +45,7 @@ constexpr int kLmM = 128;       // batch rows per tile: the TMEM lanes
 constexpr int kLmN = 128;       // vocabulary columns per tile
 constexpr int kLmBK = 64;       // K per stage: one 128-byte swizzle row of bf16
 constexpr int kLmStages = 3;      // ring stages when all 128 rows hold candidates
-constexpr int kLmStagesMax = 5;   // with only 32 rows' buffers the ring takes the rest
+constexpr int kLmStagesMax = 9;   // few rows: their buffers and boxes leave the ring more
 constexpr int kLmCap = 120;     // candidate keys buffered per row
 constexpr int kLmKeffMax = kLmCap - 32;  // a compaction leaves room for a whole chunk
 constexpr int kLmRowStride = kLmCap + 1; // odd, so rows spread over the banks
@@ -64,8 +64,9 @@ constexpr uint32_t kLmStageBytes = kLmTileABytes + kLmTileBBytes;
 constexpr uint32_t kLmRowBytes = kLmRowStride * 8;  // one row's candidate buffer
 // ns stages of A tiles, ns of B tiles, then the candidate buffers of the rows in use
 constexpr uint32_t kLmRingBytes = kLmStages * kLmStageBytes + kLmM * kLmRowBytes;
-static_assert(kLmStagesMax * kLmStageBytes + 32 * kLmRowBytes <= kLmRingBytes,
-              "the deepest ring leaves room for one warp's buffers");
+constexpr int kLmStagesWhole = 5;  // with whole boxes of xn and one warp's buffers
+static_assert(kLmStagesWhole * kLmStageBytes + 32 * kLmRowBytes <= kLmRingBytes,
+              "the deepest ring of whole boxes leaves room for one warp's buffers");
 
 struct LmSmem {  // placed at a 1024-byte boundary: the swizzled tiles need it
     uint8_t ring[kLmRingBytes];  // tiles (1024-byte aligned), then per row: keys, unordered
@@ -895,8 +896,8 @@ __device__ __forceinline__ float lm_inv_temp(float temp, const float* row_temp, 
 // The statistics of the kLmStatTiles row tiles in work, per epilogue lane: m, s and w,
 // 256 lanes apart, kLmStatFloats per row tile.
 constexpr int kLmStatFloats = 3 * 32 * kLmEpiWarps;
-static_assert(kLmStagesMax * kLmStageBytes + kLmStatTiles * kLmStatFloats * 4 <= kLmRingBytes,
-              "the statistics fit behind the deepest ring");
+static_assert(kLmStagesWhole * kLmStageBytes + kLmStatTiles * kLmStatFloats * 4 <= kLmRingBytes,
+              "the statistics fit behind a ring of whole boxes");
 __device__ __forceinline__ void lm_stat_clear(float* states) {
     for (int i = 0; i < kLmStatTiles; ++i) {
         states[i * kLmStatFloats] = -INFINITY;
@@ -947,8 +948,9 @@ __global__ void __launch_bounds__(kLmThreads, 1)
 
     const int ns = a.ns;
     uint8_t* const tiles_a = sm.ring;
-    uint8_t* const tiles_b = sm.ring + (size_t)ns * kLmTileABytes;
-    uint64_t* const cand = reinterpret_cast<uint64_t*>(sm.ring + (size_t)ns * kLmStageBytes);
+    const uint32_t a_bytes = (uint32_t)a.a_rows * kLmBK * 2;  // of a box of xn
+    uint8_t* const tiles_b = sm.ring + (size_t)ns * a_bytes;
+    uint64_t* const cand = reinterpret_cast<uint64_t*>(tiles_b + (size_t)ns * kLmTileBBytes);
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < ns; ++s) {
@@ -984,7 +986,6 @@ __global__ void __launch_bounds__(kLmThreads, 1)
     int u_begin, u_end, u_step;
     lm_range<P, STATS>(a, u_begin, u_end, u_step);
     if (STATS) grid_dep_trigger();  // zs_lm_logprob_kernel waits for this grid
-    const uint32_t a_bytes = (uint32_t)a.a_rows * kLmBK * 2;  // of a box of xn
 
     // Launched behind zs_lm_rmsnorm_kernel as a programmatic dependent: the copy
     // issuer first pulls its first weight boxes into L2 (they do not depend on the
@@ -1019,7 +1020,7 @@ __global__ void __launch_bounds__(kLmThreads, 1)
                         }
                         if (P == 1) {
                             mbar_arrive_expect_tx(&sm.full[stage], a_bytes + kLmTileBBytes);
-                            tma_load_2d(tiles_a + stage * kLmTileABytes, &tm_a, kb * kLmBK,
+                            tma_load_2d(tiles_a + stage * a_bytes, &tm_a, kb * kLmBK,
                                         m * kLmM, &sm.full[stage]);
                             tma_load_2d(tiles_b + stage * kLmTileBBytes, &tm_b, kb * kLmBK,
                                         t * kLmN, &sm.full[stage]);
@@ -1030,7 +1031,7 @@ __global__ void __launch_bounds__(kLmThreads, 1)
                                 mbar_arrive_expect_tx(&sm.full[stage],
                                                       2u * (a_bytes + kLmTileBBytes));
                             const uint32_t bar = smem_in_cta(&sm.full[stage], 0u);
-                            tma_load_2d_pair(tiles_a + stage * kLmTileABytes, &tm_a, kb * kLmBK,
+                            tma_load_2d_pair(tiles_a + stage * a_bytes, &tm_a, kb * kLmBK,
                                              m * G::kRows + (int)rank * kLmM, bar);
                             tma_load_2d_pair(tiles_b + stage * kLmTileBBytes, &tm_b, kb * kLmBK,
                                              t * G::kCols + (int)rank * kLmN, bar);
@@ -1078,7 +1079,7 @@ __global__ void __launch_bounds__(kLmThreads, 1)
                             break;
                         }
                         tc_fence_after();
-                        const uint64_t ad = sw128_desc(tiles_a + stage * kLmTileABytes);
+                        const uint64_t ad = sw128_desc(tiles_a + stage * a_bytes);
                         const uint64_t bd = sw128_desc(tiles_b + stage * kLmTileBBytes);
 #pragma unroll
                         for (int k = 0; k < kLmBK / 16; ++k) {
